@@ -344,6 +344,7 @@ def _prepare_logits(s, c, r):
         p = {k: s[k].data_ptr() for k in ("tokens", "repetition", "frequency", "presence")}
         if nb:
             p.update({k: s[k].data_ptr() for k in ("bias_offsets", "bias_ids", "bias_values")})
+            p.update(biases=nb * rows)
         if m:
             p.update(mask=s["mask"].data_ptr(), mask_index=s["mask_index"].data_ptr(),
                      mask_stride=words, masks=m)
