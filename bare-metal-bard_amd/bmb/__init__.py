@@ -74,6 +74,47 @@ class GPT(ctypes.Structure):
 
 _GPTP = ctypes.POINTER(GPT)
 
+# Element types of the paged cache and of logits_process (include/flash.h, nn.h).
+F32, F16, BF16 = 0, 1, 2
+ELEMENT_TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+
+
+class PagedCache(ctypes.Structure):
+    """Mirror of `struct PagedCache` (include/flash.h). Pointers are device
+    addresses; the caller keeps the buffers alive (here and below)."""
+    _fields_ = ([("k", c_vp), ("v", c_vp)]
+                + [(n, c_int) for n in ("type", "pages", "page_size", "kv_heads", "head_size")]
+                + [(n, c_ll) for n in ("page_stride", "token_stride", "head_stride")])
+
+
+class PagedPlan(ctypes.Structure):
+    """Mirror of `struct PagedPlan` (include/flash.h)."""
+    _fields_ = ([(n, c_int) for n in ("requests", "max_pages", "pages", "page_size", "max_tokens")]
+                + [(n, c_vp) for n in ("new_tokens", "lens", "lens_out", "state", "state_out",
+                                       "free_pages", "block_table", "slots", "positions", "rows",
+                                       "offsets")])
+
+
+class PagedBatch(ctypes.Structure):
+    """Mirror of `struct PagedBatch` (include/flash.h)."""
+    _fields_ = ([(n, c_int) for n in ("requests", "max_len", "table_stride", "heads", "n_rows",
+                                      "type")]
+                + [("scale", c_float), ("q_stride", c_ll), ("out_stride", c_ll)]
+                + [(n, c_vp) for n in ("block_table", "lens", "rows", "work")]
+                + [("work_bytes", c_size_t)])
+
+
+class LogitsRules(ctypes.Structure):
+    """Mirror of `struct LogitsRules` (include/nn.h); a field left out is null."""
+    _fields_ = ([("tokens", c_vp), ("token_stride", c_ll)]
+                + [(n, c_vp) for n in ("lens", "prompt_lens", "repetition", "frequency",
+                                       "presence", "bias_offsets", "bias_ids", "bias_values")]
+                + [("biases", c_int), ("masks", c_int), ("mask", c_vp), ("mask_stride", c_ll),
+                   ("mask_index", c_vp)])
+
+
+_CACHEP, _BATCHP = ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch)
+
 # Every symbol the C headers declare, with its ctypes signature.
 _SIGS = {
     # kernels.h
@@ -112,6 +153,10 @@ _SIGS = {
     "flash_default_bwd_config": (c_int, []),
     "flash_attention_backward_cfg": (c_bool, [c_int, c_vp, c_vp, c_vp, c_vp, c_vp,
                                               c_vp, c_int, c_int, c_int, c_int]),
+    "paged_plan": (c_int, [ctypes.POINTER(PagedPlan), c_vp]),
+    "paged_append": (c_int, [_CACHEP, c_vp, c_vp, c_int, c_ll, c_vp, c_int, c_vp]),
+    "paged_attention_workspace": (c_size_t, [_CACHEP, _BATCHP]),
+    "paged_attention": (c_int, [_CACHEP, _BATCHP, c_vp, c_vp, c_vp, c_vp]),
     # attention.h
     "attention_forward": (None, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int]),
     "attention_backward": (None, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int,
@@ -136,6 +181,8 @@ _SIGS = {
     "grad_global_norm": (c_float, [c_vp, c_int]),
     "zero_buffer": (None, [c_vp, c_size_t]),
     "reduce_mean": (c_float, [c_vp, c_int]),
+    "logits_process": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_ll,
+                               ctypes.POINTER(LogitsRules), c_vp]),
     # gpt.h
     "param_sizes": (None, [ctypes.POINTER(c_size_t), ctypes.POINTER(GPTConfig)]),
     "gpt_alloc": (None, [_GPTP]),
@@ -296,7 +343,33 @@ def flash_default_bwd_config() -> int:
     return int(lib().flash_default_bwd_config())
 
 
+# Generation (the paged key-value cache). A call that the library refuses
+# raises; the library's message, on stderr, says why.
+def paged_plan(plan: PagedPlan, stream=0) -> None:
+    if (_lib or lib()).paged_plan(plan, stream or None):
+        raise ValueError("paged_plan refused its arguments")
+
+
+def paged_append(cache: PagedCache, k, v, type, row_stride, slots, tokens, stream=0) -> None:
+    if (_lib or lib()).paged_append(cache, k, v, type, row_stride, slots, tokens, stream or None):
+        raise ValueError("paged_append refused its arguments")
+
+
+def paged_attention_workspace(cache: PagedCache, batch: PagedBatch) -> int:
+    return lib().paged_attention_workspace(cache, batch)
+
+
+def paged_attention(cache: PagedCache, batch: PagedBatch, out, lse, q, stream=0) -> None:
+    if (_lib or lib()).paged_attention(cache, batch, out, lse, q, stream or None):
+        raise ValueError("paged_attention refused its arguments")
+
+
 # ------------------------------------------------------------ attention.h / nn.h
+def logits_process(out, logits, type, rows, V, stride, rules: LogitsRules, stream=0) -> None:
+    if (_lib or lib()).logits_process(out, logits, type, rows, V, stride, rules, stream or None):
+        raise ValueError("logits_process refused its arguments")
+
+
 def call(name, *args):
     """Calls the C entry point `name` with raw arguments (device pointers as
     ints); returns its result."""

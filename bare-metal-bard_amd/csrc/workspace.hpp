@@ -39,7 +39,8 @@ enum ScratchSlot {
     SCRATCH_FLASH_DS = 0,  // flash backward dS tiles
     SCRATCH_NN = 1,        // nn.h reductions (partials, scalar results)
     SCRATCH_GEMM = 2,      // split-K partial sums of gemm()
-    SCRATCH_SLOTS = 3
+    SCRATCH_PAGED = 3,     // partial results of paged_attention()
+    SCRATCH_SLOTS = 4
 };
 
 struct ScratchBuffer;

@@ -26,6 +26,15 @@
 
 #include <stddef.h>
 
+struct ihipStream_t; /* hipStream_t is a pointer to it */
+
+/* Element types of logits_process and of the paged cache (flash.h). */
+#ifndef BMB_F32
+#define BMB_F32 0
+#define BMB_F16 1
+#define BMB_BF16 2
+#endif
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -99,6 +108,41 @@ void zero_buffer(float *p, size_t n);
 /* Mean of n device floats, accumulated in fp64; blocks until the result is
  * on the host. */
 float reduce_mean(const float *d_values, int n);
+
+/* ---- sampling: what stands between the logits and a choice of token ----
+ * No counterpart in the reference. Rules that a null pointer leaves out do
+ * nothing. In this order, on row r's logit x of token id i (fp32 arithmetic,
+ * one rounding at the end):
+ *   penalties for the row's first lens[r] tokens, of which the first
+ *   prompt_lens[r] are its prompt and the others its output:
+ *     repetition[r]: x > 0 ? x / rep : x * rep if i is among them;
+ *     frequency[r]: x - f * (times that i is in the output);
+ *     presence[r]: x - p if i is in the output;
+ *   a bias: x + value for i in the row's list (the last entry of an id counts);
+ *   a grammar's mask: -inf where bit i%32 of word i/32 is 0, whatever x was.
+ * Token ids outside [0, V) are ignored. */
+typedef struct LogitsRules {
+    const int *tokens;      /* (rows, token_stride) */
+    long long token_stride; /* lens[r] is read as if clipped to [0, token_stride] */
+    const int *lens, *prompt_lens;                /* (rows); prompt_lens null: all 0 */
+    const float *repetition, *frequency, *presence; /* (rows) */
+    const int *bias_offsets; /* (rows + 1): row r's entries are [offsets[r], offsets[r+1]) */
+    const int *bias_ids;     /* (biases) */
+    const float *bias_values;
+    int biases;              /* entries in all; offsets are clipped to [0, biases] */
+    int masks;               /* masks given */
+    const unsigned *mask;    /* (masks, mask_stride) words, at least ceil(V / 32) a mask */
+    long long mask_stride;
+    const int *mask_index;   /* (rows): its mask, or any number outside [0, masks) for none;
+                                null: row r has mask r (masks >= rows) */
+} LogitsRules;
+/* out = logits under the rules, both (rows, V) of `type` (BMB_F32, BMB_F16 or
+ * BMB_BF16) with `stride` elements from row to row; columns [V, stride) are
+ * left as they were. out may be logits; other overlaps are not allowed.
+ * Queued on `stream`; returns 0, or -1 with a message on stderr, and nothing
+ * launched, for arguments it refuses. Allocates nothing. */
+int logits_process(void *out, const void *logits, int type, int rows, int V, long long stride,
+                   const LogitsRules *rules, struct ihipStream_t *stream);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus
