@@ -21,6 +21,8 @@
 //                 memory; product j takes element j of each lane's.
 // So neither the probabilities nor the values pass through LDS, and loads are
 // whole rows.
+#include <optional>
+
 #include "launch.hpp"
 #include "paged.hpp"
 #include "workspace.hpp"
@@ -28,7 +30,7 @@
 namespace bmb {
 namespace {
 
-constexpr int WAVES = 4, THREADS = WAVES * WAVE, COLS = 16;
+constexpr int COLS = 16;
 constexpr int UNIT = 128;  // a part is a whole number of these keys
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -48,13 +50,18 @@ struct AttendArgs {
     int requests, heads, kv_heads, group, tiles, pages, table_stride, max_len, n_rows;
     int slots;     // parts that the launch has room for
     int workers;   // parts aimed at; 0: one part a request
+    int few;       // parts at one workgroup a CU
+    int least, enough;  // units of a part: at least, and no fewer parts than `few` for more
+    int cached;    // units from which on a batch passes the caches
     float scale;   // times log2(e)
     FastDiv page;
+    uint32_t page16, token16;  // strides in units of 16 bytes
 };
 
 // The part of a request that a slot stands for; n: how many the request has (0: none here).
 struct Part {
     int r, i, n, begin, end, row;
+    bool nt;  // the step's batch passes the caches
 };
 
 __device__ __forceinline__ int row_of(const AttendArgs &a, int r) {
@@ -72,7 +79,7 @@ __device__ __forceinline__ int len_of(const AttendArgs &a, int r) {
 // its slot's request by itself, 64 requests at a time.
 __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
-    Part p = {slot, 0, 0, 0, 0, -1};
+    Part p = {slot, 0, 0, 0, 0, -1, a.cached == 0};
     if (a.workers == 0) {
         p.row = row_of(a, slot);
         p.n = p.row >= 0;
@@ -86,7 +93,10 @@ __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
         if (r < a.requests && row_of(a, r) >= 0) units = (len_of(a, r) + UNIT - 1) / UNIT;
         total += __builtin_amdgcn_readlane(wave_scan(units), 63);
     }
-    const uint32_t size = max((total + a.workers - 1) / a.workers, 1u);
+    p.nt = total >= (uint32_t)a.cached;
+    uint32_t size = (total + a.workers - 1) / a.workers;
+    size = max(size, min((total + a.few - 1) / a.few, (uint32_t)a.enough));
+    size = max(size, (uint32_t)a.least);
     uint32_t before = 0;
     for (int base = 0; base < a.requests; base += WAVE) {
         const int r = base + lane;
@@ -140,6 +150,16 @@ __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// A load of the cache. NT: not kept in the caches behind it (non-temporal), for
+// batches that do not fit them anyway.
+template <bool NT, typename R>
+__device__ __forceinline__ R load(const char *p) {
+    if constexpr (NT)
+        return __builtin_nontemporal_load((const R *)p);
+    else
+        return *(const R *)p;
+}
+
 // What a wave holds of the queries and of one step's keys and values, and the
 // two products on it. TILES groups of 16 keys a step.
 //
@@ -151,6 +171,7 @@ __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
 template <typename T, int HS>
 struct Half {
     using Q = T;
+    static constexpr int SIZE = sizeof(T);
     static constexpr int TILES = 2, KV = 4 * TILES, DPL = HS / 16;
     using V8 = vec<T, 8>;
     using Row = vec<uint32_t, DPL / 2>;
@@ -168,12 +189,14 @@ struct Half {
     static __device__ __forceinline__ void zero_q(Query &q) {
         for (int s = 0; s < HS / 32; ++s) q.q[s] = (V8)(T)0.0f;
     }
+    template <bool NT>
     static __device__ __forceinline__ void load_k(Regs &x, int t, const char *row, int g) {
         for (int s = 0; s < HS / 32; ++s)
-            x.k[t][s] = *(const V8 *)(row + (s * 32 + g * 8) * sizeof(T));
+            x.k[t][s] = load<NT, V8>(row + (s * 32 + g * 8) * sizeof(T));
     }
+    template <bool NT>
     static __device__ __forceinline__ void load_v(Regs &x, int i, const char *row, int c) {
-        x.v[i] = *(const Row *)(row + c * DPL * sizeof(T));
+        x.v[i] = load<NT, Row>(row + c * DPL * sizeof(T));
     }
     static __device__ __forceinline__ void zero_v(Regs &x, int i) { x.v[i] = (Row)0u; }
     static __device__ __forceinline__ f32x4 scores(const Regs &x, int t, const Query &q) {
@@ -210,7 +233,9 @@ struct Half {
 template <typename T, int HS>
 struct Full {
     using Q = float;
-    static constexpr int TILES = 1, KV = 4, DPL = HS / 16;
+    static constexpr int SIZE = sizeof(T);
+    // (32 keys of 16-bit heads of 128 take too many registers: 64 -> 82 us.)
+    static constexpr int TILES = sizeof(T) == 2 && HS <= 64 ? 2 : 1, KV = 4 * TILES, DPL = HS / 16;
     static constexpr int EPL = 16 / sizeof(T);  // elements of a 16-byte load
     using VE = vec<T, EPL>;
     struct Query {
@@ -231,12 +256,14 @@ struct Full {
     static __device__ __forceinline__ void zero_q(Query &q) {
         for (int s = 0; s < HS / 4; ++s) q.q[s] = 0.0f;
     }
+    template <bool NT>
     static __device__ __forceinline__ void load_k(Regs &x, int t, const char *row, int g) {
         for (int s = 0; s < HS / (4 * EPL); ++s)
-            x.k[t][s] = *(const VE *)(row + (s * 4 + g) * 16);
+            x.k[t][s] = load<NT, VE>(row + (s * 4 + g) * 16);
     }
+    template <bool NT>
     static __device__ __forceinline__ void load_v(Regs &x, int i, const char *row, int c) {
-        x.v[i] = *(const vec<T, DPL> *)(row + c * DPL * sizeof(T));
+        x.v[i] = load<NT, vec<T, DPL>>(row + c * DPL * sizeof(T));
     }
     static __device__ __forceinline__ void zero_v(Regs &x, int i) {
         x.v[i] = (vec<T, DPL>)(T)0.0f;
@@ -258,92 +285,141 @@ struct Full {
     }
 };
 
+// The pages of one step's keys, read one step ahead of their rows. ALIGNED: 16
+// keys from a multiple of 16 on lie in one page, so a page id is read once a
+// tile, by the scalar unit. Otherwise each lane looks up one of the step's keys
+// and the lanes exchange the rows' places (in units of 16 bytes, as every
+// stride is a multiple of that): with every lane looking up the pages of its
+// own rows, pages of 24 keys took 137 us where pages of 16 took 99 (16
+// sequences of 16000 keys, 4 heads of 128, bf16).
+constexpr uint32_t NO_ROW = 0xffffffffu;
+template <bool ALIGNED, int TILES>
+struct Pages {
+    int id[ALIGNED ? TILES : 1];
+    __device__ __forceinline__ void fetch(const AttendArgs &a, const int *table, int kb, int end) {
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+                id[t] = kb + 16 * t < end ? table[a.page.quot(kb + 16 * t)] : -1;
+        } else {
+            const int key = kb + (int)(threadIdx.x & (16 * TILES - 1));
+            id[0] = key < end ? table[a.page.quot(key)] : -1;
+        }
+    }
+    // Not ALIGNED: the place of this lane's key.
+    __device__ __forceinline__ uint32_t place(const AttendArgs &a, int kb) const {
+        const int key = kb + (int)(threadIdx.x & (16 * TILES - 1));
+        const uint32_t in = key - a.page.quot(key) * (int)a.page.d;
+        return (unsigned)id[0] < (unsigned)a.pages ? id[0] * a.page16 + in * a.token16 : NO_ROW;
+    }
+    // ALIGNED: the place of a tile's first key, and how many of it count (none:
+    // the first rows of the cache, which are left out).
+    __device__ __forceinline__ void tile(const AttendArgs &a, int t, int kb, int end, int esize,
+                                         int &n, long long &at) const {
+        const int base = kb + 16 * t;
+        n = (unsigned)id[t] < (unsigned)a.pages ? min(end - base, 16) : 0;
+        const int in = base - a.page.quot(base) * (int)a.page.d;
+        at = n > 0 ? (id[t] * a.page_stride + in * a.token_stride) * esize : 0;
+    }
+};
+
 // Loads the step of keys from kb on. Returns which of the lane's KV keys (4g +
-// r of each 16) count. ALIGNED: 16 keys from a multiple of 16 on lie in one
-// page, so a page id is read once, by the scalar unit, and keys behind `end`
-// are read (inside their page) and left out; otherwise each lane looks its
-// own keys' pages up.
-template <typename P, bool ALIGNED>
+// r of each 16) count. Keys behind `end` are read where their page goes on, or
+// from the first row, and left out.
+template <typename P, bool ALIGNED, bool NT>
 __device__ __forceinline__ unsigned load_step(typename P::Regs &x, const AttendArgs &a,
-                                              const int *table, const char *k, const char *v,
-                                              int esize, int kb, int end, int g, int c) {
+                                              const Pages<ALIGNED, P::TILES> &pages,
+                                              const char *k, const char *v, int kb, int end, int g,
+                                              int c) {
     unsigned live = 0;
+    uint32_t place = 0;
+    if constexpr (!ALIGNED) place = pages.place(a, kb);
 #pragma unroll
     for (int t = 0; t < P::TILES; ++t) {
-        const int base = kb + 16 * t;
         if constexpr (ALIGNED) {
-            const int b = base < end ? base : 0;
-            const int j = a.page.quot(b);
-            int page = base < end ? table[j] : -1;
-            const int n = (unsigned)page < (unsigned)a.pages ? min(end - base, 16) : 0;
-            page = n > 0 ? page : 0;
-            const long long at = page * a.page_stride + (b - j * (int)a.page.d) * a.token_stride;
-            P::load_k(x, t, k + (at + c * a.token_stride) * esize, g);
+            int n;
+            long long at;
+            pages.tile(a, t, kb, end, P::SIZE, n, at);
+            const long long row = a.token_stride * P::SIZE;
+            P::template load_k<NT>(x, t, k + at + c * row, g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                P::load_v(x, 4 * t + r, v + (at + (4 * g + r) * a.token_stride) * esize, c);
+                P::template load_v<NT>(x, 4 * t + r, v + at + (4 * g + r) * row, c);
                 live |= (4 * g + r < n ? 1u : 0u) << (4 * t + r);
             }
         } else {
-            const auto find = [&](int key, bool &ok) {
-                const int n = key < end ? key : 0;
-                const int j = a.page.quot(n);
-                int page = key < end ? table[j] : -1;
-                ok = (unsigned)page < (unsigned)a.pages;
-                page = ok ? page : 0;
-                return page * a.page_stride + (n - j * (int)a.page.d) * a.token_stride;
-            };
-            bool ok;
-            P::load_k(x, t, k + find(base + c, ok) * esize, g);
+            const uint32_t at = __shfl(place, 16 * t + c);
+            P::template load_k<NT>(x, t, k + (at == NO_ROW ? 0ull : at * 16ull), g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                P::load_v(x, 4 * t + r, v + find(base + 4 * g + r, ok) * esize, c);
-                live |= (ok ? 1u : 0u) << (4 * t + r);
+                const uint32_t to = __shfl(place, 16 * t + 4 * g + r);
+                P::template load_v<NT>(x, 4 * t + r, v + (to == NO_ROW ? 0ull : to * 16ull), c);
+                live |= (to != NO_ROW ? 1u : 0u) << (4 * t + r);
             }
         }
     }
     return live;
 }
 
-template <template <typename, int> class POLICY, typename TC, int HS, bool ALIGNED>
-__global__ __launch_bounds__(THREADS) void attend_kernel(AttendArgs a) {
-    using P = POLICY<TC, HS>;
-    using TQ = typename P::Q;
-    constexpr int STEP = 16 * P::TILES, DPL = P::DPL, KV = P::KV;
-    __shared__ float part_ml[WAVES][2][COLS];
-    __shared__ float part_o[WAVES][COLS][HS];
+// LDS of a workgroup: each wave's running maxima and sums, and its share of
+// the result for the columns in use.
+constexpr size_t merge_bytes(int waves, int cols, int hs) {
+    return (size_t)waves * (2 * COLS + cols * hs) * sizeof(float);
+}
 
-    // Workgroups go to the XCDs in turn: all heads of a slot on one of them,
-    // since rows of neighbouring heads can share cache lines.
-    const int per = 8 * a.kv_heads * a.tiles;
-    const int in = blockIdx.x % per, slot = blockIdx.x / per * 8 + in % 8;
-    if (slot >= a.slots) return;
-    const int kv_head = in / 8 / a.tiles, tile = in / 8 % a.tiles;
-    const Part part = find_part(a, slot);
-    if (part.n == 0) return;
-
-    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cols = min(a.group - tile * COLS, COLS);
-    const int head0 = kv_head * a.group + tile * COLS;  // the first query head here
-    const int *table = a.table + (size_t)part.r * a.table_stride;
-    const char *k = a.k + kv_head * a.head_stride * (long long)sizeof(TC);
-    const char *v = a.v + kv_head * a.head_stride * (long long)sizeof(TC);
-
-    typename P::Query q;
-    if (c < cols)
-        P::load_q(q, (const TQ *)a.q + part.row * a.q_stride + (head0 + c) * HS, g);
-    else
-        P::zero_q(q);
-
-    f32x4 o[DPL];
+// The waves' results, each weighed by its maximum: to the result, or as a part
+// of a split request.
+template <typename TQ, int HS, int WAVES>
+__device__ __forceinline__ void merge_waves(const AttendArgs &a, const Part &part, int slot,
+                                            int head0, int cols) {
+    extern __shared__ float merge[];
+    const float(*part_ml)[2][COLS] = (const float(*)[2][COLS])merge;
+    const float *part_o = merge + WAVES * 2 * COLS;
+    __syncthreads();
+    for (int i = threadIdx.x; i < cols * HS; i += WAVES * WAVE) {
+        const int col = i / HS, d = i % HS;
+        float top = part_ml[0][0][col];
 #pragma unroll
-    for (int j = 0; j < DPL; ++j) o[j] = {0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;  // of column c; l of this lane's keys only
-    for (int kb = part.begin + wave * STEP; kb < part.end; kb += WAVES * STEP) {
+        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, part_ml[w][0][col]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f(part_ml[w][0][col] - ref);
+            sum += f * part_ml[w][1][col];
+            acc += f * part_o[w * cols * HS + i];
+        }
+        const int head = head0 + col;
+        if (part.n == 1) {
+            const float y = sum == 0.0f ? 0.0f : acc / sum;
+            ((TQ *)a.out)[part.row * a.out_stride + head * HS + d] = (TQ)y;
+            if (a.lse && d == 0)
+                a.lse[(long long)part.row * a.heads + head] =
+                    sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
+        } else {
+            const long long at = (long long)slot * a.heads + head;
+            a.part_o[at * HS + d] = acc;
+            if (d == 0) a.part_ml[at] = make_float2(top, sum);
+        }
+    }
+    if (a.workers && threadIdx.x == 0 && part.i == 0 && head0 == 0)
+        a.parts[part.r] = make_int2(slot, part.n);
+}
+
+// A wave's share of a part: steps of keys from `first` on, `step` apart.
+template <typename P, bool ALIGNED, bool NT>
+__device__ __forceinline__ void attend_steps(f32x4 (&o)[P::DPL], float &m, float &l,
+                                             const AttendArgs &a, const Part &part,
+                                             const typename P::Query &q, const int *table,
+                                             const char *k, const char *v, int first, int step,
+                                             int g, int c) {
+    constexpr int DPL = P::DPL, KV = P::KV;
+    Pages<ALIGNED, P::TILES> pages, next;
+    pages.fetch(a, table, part.begin + first, part.end);
+    for (int kb = part.begin + first; kb < part.end; kb += step, pages = next) {
         typename P::Regs x;
-        const unsigned live =
-            load_step<P, ALIGNED>(x, a, table, k, v, sizeof(TC), kb, part.end, g, c);
+        next.fetch(a, table, kb + step, part.end);
+        const unsigned live = load_step<P, ALIGNED, NT>(x, a, pages, k, v, kb, part.end, g, c);
         const bool whole = __builtin_amdgcn_ballot_w64(live != (1u << KV) - 1) == 0;
         float p[KV];
 #pragma unroll
@@ -380,10 +456,51 @@ __global__ __launch_bounds__(THREADS) void attend_kernel(AttendArgs a) {
         for (int j = 0; j < DPL; ++j) o[j] *= keep;
         P::values(o, x, p);
     }
+}
+
+template <template <typename, int> class POLICY, typename TC, int HS, bool ALIGNED>
+__global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
+    using P = POLICY<TC, HS>;
+    using TQ = typename P::Q;
+    constexpr int WAVES = 4, STEP = 16 * P::TILES, DPL = P::DPL;
+    extern __shared__ float merge[];
+    float(*part_ml)[2][COLS] = (float(*)[2][COLS])merge;
+    float *part_o = merge + WAVES * 2 * COLS;  // (wave, column, element)
+
+    // Workgroups go to the XCDs in turn: all heads of a slot on one of them,
+    // since rows of neighbouring heads can share cache lines.
+    const int per = 8 * a.kv_heads * a.tiles;
+    const int in = blockIdx.x % per, slot = blockIdx.x / per * 8 + in % 8;
+    if (slot >= a.slots) return;
+    const int kv_head = in / 8 / a.tiles, tile = in / 8 % a.tiles;
+    const Part part = find_part(a, slot);
+    if (part.n == 0) return;
+
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cols = min(a.group - tile * COLS, COLS);
+    const int head0 = kv_head * a.group + tile * COLS;  // the first query head here
+    const int *table = a.table + (size_t)part.r * a.table_stride;
+    const char *k = a.k + kv_head * a.head_stride * (long long)sizeof(TC);
+    const char *v = a.v + kv_head * a.head_stride * (long long)sizeof(TC);
+
+    typename P::Query q;
+    if (c < cols)
+        P::load_q(q, (const TQ *)a.q + part.row * a.q_stride + (head0 + c) * HS, g);
+    else
+        P::zero_q(q);
+
+    f32x4 o[DPL];
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) o[j] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;  // of column c; l of this lane's keys only
+    if (part.nt)
+        attend_steps<P, ALIGNED, true>(o, m, l, a, part, q, table, k, v, wave * STEP, WAVES * STEP, g, c);
+    else
+        attend_steps<P, ALIGNED, false>(o, m, l, a, part, q, table, k, v, wave * STEP, WAVES * STEP, g, c);
     l = col_sum(l);
 
-    // The four waves' results through LDS; the first to read a column's
-    // maxima weighs each wave's share.
+    // The waves' results through LDS, each weighed by its maximum.
     if (g == 0) {
         part_ml[wave][0][c] = m;
         part_ml[wave][1][c] = l;
@@ -392,79 +509,286 @@ __global__ __launch_bounds__(THREADS) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < DPL; ++j) part_o[wave][c][(4 * g + r) * DPL + j] = o[j][r];
+            for (int j = 0; j < DPL; ++j)
+                part_o[(wave * cols + c) * HS + (4 * g + r) * DPL + j] = o[j][r];
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < cols * HS; i += THREADS) {
-        const int col = i / HS, d = i % HS;
-        float top = part_ml[0][0][col];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, part_ml[w][0][col]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, acc = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const float f = __builtin_amdgcn_exp2f(part_ml[w][0][col] - ref);
-            sum += f * part_ml[w][1][col];
-            acc += f * part_o[w][col][d];
-        }
-        const int head = head0 + col;
-        if (part.n == 1) {
-            const float y = sum == 0.0f ? 0.0f : acc / sum;
-            ((TQ *)a.out)[part.row * a.out_stride + head * HS + d] = (TQ)y;
-            if (a.lse && d == 0)
-                a.lse[(long long)part.row * a.heads + head] =
-                    sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
-        } else {
-            const long long at = (long long)slot * a.heads + head;
-            a.part_o[at * HS + d] = acc;
-            if (d == 0) a.part_ml[at] = make_float2(top, sum);
-        }
-    }
-    if (a.workers && threadIdx.x == 0 && part.i == 0 && kv_head == 0 && tile == 0)
-        a.parts[part.r] = make_int2(slot, part.n);
+    merge_waves<TQ, HS, WAVES>(a, part, slot, head0, cols);
 }
 
-// Joins the parts of split requests: one workgroup a request and head.
+// ---- few query heads to a kv head, fp32 queries: 16 matrix columns would
+// mostly be empty, and fp32 matrix instructions have no rate to spare (12
+// heads, 1000 keys of 64: 16.9 us with them). Sixteen lanes take a key, each
+// HS/16 of its elements, so a wave's load is four whole rows; KEYS loads make a
+// step, lane (g, c) with keys 4 i + g. A key's partial sums are added over its
+// lanes while they are spread over them (half of the keys kept, half sent, at
+// each step), which leaves lane c with the score of key i = c mod KEYS; the
+// probabilities come back for the values' sums as broadcasts of a lane over
+// its row of 16. Each row of 16 lanes keeps its own running maximum.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, XOR7 = 0x141, ROR4 = 0x124, ROR8 = 0x128;
+
+// s[0..N-1] of each lane to the sums over lanes: lanes whose `up` bit is set
+// keep the upper half.
+template <int CTRL, int N>
+__device__ __forceinline__ void halve(float *s, bool up) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const float keep = up ? s[i + N / 2] : s[i], send = up ? s[i] : s[i + N / 2];
+        s[i] = keep + dpp<CTRL>(send);
+    }
+}
+// (The partners 8, 7, 2 and 1 apart, as exclusive or, reach all sixteen lanes,
+// and each pair still holds the same keys when it meets.)
+template <int KEYS>
+__device__ __forceinline__ float spread_sum(float (&s)[KEYS], int c) {
+    if constexpr (KEYS == 16) halve<ROR8, 16>(s, c & 8);
+    if constexpr (KEYS >= 8) halve<XOR7, 8>(s, c & 4);
+    halve<XOR2, 4>(s, c & 2);
+    halve<XOR1, 2>(s, c & 1);
+    float x = s[0];
+    if constexpr (KEYS == 4) x += dpp<ROR4>(x);
+    if constexpr (KEYS <= 8) x += dpp<ROR8>(x);
+    return x;
+}
+template <int KEYS>
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, dpp<XOR1>(x));
+    x = fmaxf(x, dpp<XOR2>(x));
+    if constexpr (KEYS >= 8) x = fmaxf(x, dpp<XOR7>(x));
+    if constexpr (KEYS == 16) x = fmaxf(x, dpp<ROR8>(x));
+    return x;
+}
+
+template <int I, int KEYS, int DPL, typename Row>
+__device__ __forceinline__ void add_values(float *acc, float p, const Row (&v)[KEYS]) {
+    if constexpr (I < KEYS) {
+        const float w = dpp<0x150 + I>(p);
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) acc[j] = fma_rn(w, (float)v[I][j], acc[j]);
+        add_values<I + 1, KEYS, DPL>(acc, p, v);
+    }
+}
+
+// Lane c's HS/16 elements of a row: contiguous, or two pieces of 16 bytes half a
+// row apart, so that each load covers whole lines.
+template <typename T, int HS>
+__device__ __forceinline__ constexpr int row_at(int c, int j) {
+    constexpr int DPL = HS / 16, E = 16 / sizeof(T);
+    return DPL <= E ? c * DPL + j : (j / E) * (HS / 2) + c * E + j % E;
+}
+template <typename T, int HS, bool NT>
+__device__ __forceinline__ vec<T, HS / 16> load_row(const char *p) {
+    constexpr int DPL = HS / 16, E = 16 / sizeof(T);
+    if constexpr (DPL <= E) {
+        return load<NT, vec<T, DPL>>(p);
+    } else {
+        const vec<T, E> x = load<NT, vec<T, E>>(p);
+        const vec<T, E> y = load<NT, vec<T, E>>(p + HS / 2 * sizeof(T));
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// A step's rows of K and V, and which of the lane's keys (kb + 4 i + g) count; as
+// load_step.
+template <typename T, int HS, int KEYS, bool ALIGNED, bool NT>
+__device__ __forceinline__ unsigned load_rows(vec<T, HS / 16> (&kr)[KEYS],
+                                              vec<T, HS / 16> (&vr)[KEYS], const AttendArgs &a,
+                                              const Pages<ALIGNED, KEYS / 4> &pages,
+                                              const char *k, const char *v, int kb, int end,
+                                              int g) {
+    unsigned live = 0;
+    if constexpr (ALIGNED) {
+#pragma unroll
+        for (int t = 0; t < KEYS / 4; ++t) {
+            int n;
+            long long at;
+            pages.tile(a, t, kb, end, sizeof(T), n, at);
+            const long long row = a.token_stride * (int)sizeof(T);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const long long to = at + (4 * r + g) * row;
+                kr[4 * t + r] = load_row<T, HS, NT>(k + to);
+                vr[4 * t + r] = load_row<T, HS, NT>(v + to);
+                live |= (4 * r + g < n ? 1u : 0u) << (4 * t + r);
+            }
+        }
+    } else {
+        const uint32_t place = pages.place(a, kb);
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) {
+            const uint32_t at = __shfl(place, 4 * i + g);
+            const unsigned long long to = at == NO_ROW ? 0ull : at * 16ull;
+            kr[i] = load_row<T, HS, NT>(k + to);
+            vr[i] = load_row<T, HS, NT>(v + to);
+            live |= (at != NO_ROW ? 1u : 0u) << i;
+        }
+    }
+    return live;
+}
+
+template <typename T, int HS, int G, int KEYS, bool ALIGNED, bool NT>
+__device__ __forceinline__ void rows_steps(float (&acc)[G][HS / 16], float (&m)[G], float (&l)[G],
+                                           const AttendArgs &a, const Part &part,
+                                           const float (&q)[G][HS / 16], const int *table,
+                                           const char *k, const char *v, int first, int step,
+                                           int g, int c) {
+    constexpr int DPL = HS / 16;
+    using Row = vec<T, DPL>;
+    Pages<ALIGNED, KEYS / 4> pages, next;
+    pages.fetch(a, table, part.begin + first, part.end);
+    for (int kb = part.begin + first; kb < part.end; kb += step, pages = next) {
+        Row kr[KEYS], vr[KEYS];
+        next.fetch(a, table, kb + step, part.end);
+        const unsigned live =
+            load_rows<T, HS, KEYS, ALIGNED, NT>(kr, vr, a, pages, k, v, kb, part.end, g);
+        const bool whole = __builtin_amdgcn_ballot_w64(live != (1u << KEYS) - 1) == 0;
+        if (!whole) {
+            // (the value itself is replaced: 0 times an infinity is no 0)
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i)
+                if (!(live >> i & 1)) vr[i] = (Row)(T)0.0f;
+        }
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            float s[KEYS];
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) {
+                s[i] = q[h][0] * (float)kr[i][0];
+#pragma unroll
+                for (int j = 1; j < DPL; ++j) s[i] = fma_rn(q[h][j], (float)kr[i][j], s[i]);
+            }
+            float x = spread_sum<KEYS>(s, c);
+            if (!whole) x = live >> (c & (KEYS - 1)) & 1 ? x : -INFINITY;
+            const float m1 = fmaxf(m[h], row_max<KEYS>(x));
+            const float ref = m1 == -INFINITY ? 0.0f : m1;
+            const float keep = __builtin_amdgcn_exp2f(m[h] - ref);
+            const float p = __builtin_amdgcn_exp2f(x - ref);
+            m[h] = m1;
+            l[h] = l[h] * keep + p;
+#pragma unroll
+            for (int j = 0; j < DPL; ++j) acc[h][j] *= keep;
+            add_values<0, KEYS, DPL>(acc[h], p, vr);
+        }
+    }
+}
+
+template <typename T, int HS, int G, bool ALIGNED, int WAVES>
+__global__ __launch_bounds__(WAVES *WAVE) void attend_rows_kernel(AttendArgs a) {
+    constexpr int DPL = HS / 16, BYTES = DPL * sizeof(T);
+    constexpr int KEYS = BYTES >= 32 ? 4 : BYTES == 16 ? 8 : 16;  // 32 registers each of K and V
+    constexpr int STEP = 4 * KEYS;
+    extern __shared__ float merge[];
+    float(*part_ml)[2][COLS] = (float(*)[2][COLS])merge;
+    float *part_o = merge + WAVES * 2 * COLS;  // (wave, head, element)
+
+    const int per = 8 * a.kv_heads * a.tiles;
+    const int in = blockIdx.x % per, slot = blockIdx.x / per * 8 + in % 8;
+    if (slot >= a.slots) return;
+    const int kv_head = in / 8 / a.tiles, tile = in / 8 % a.tiles;
+    const Part part = find_part(a, slot);
+    if (part.n == 0) return;
+
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cols = min(a.group - tile * G, G);
+    const int head0 = kv_head * a.group + tile * G;
+    const int *table = a.table + (size_t)part.r * a.table_stride;
+    const long long lane_at = kv_head * a.head_stride + row_at<T, HS>(c, 0);
+    const char *k = a.k + lane_at * (int)sizeof(T), *v = a.v + lane_at * (int)sizeof(T);
+
+    float q[G][DPL], acc[G][DPL], m[G], l[G];
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+        const float *row = (const float *)a.q + part.row * a.q_stride +
+                           (head0 + min(h, cols - 1)) * HS;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) {
+            q[h][j] = row[row_at<T, HS>(c, j)] * a.scale;
+            acc[h][j] = 0.0f;
+        }
+        m[h] = -INFINITY;
+        l[h] = 0.0f;
+    }
+    if (part.nt)
+        rows_steps<T, HS, G, KEYS, ALIGNED, true>(acc, m, l, a, part, q, table, k, v, wave * STEP,
+                                                  WAVES * STEP, g, c);
+    else
+        rows_steps<T, HS, G, KEYS, ALIGNED, false>(acc, m, l, a, part, q, table, k, v, wave * STEP,
+                                                   WAVES * STEP, g, c);
+    // The four rows of the wave into one.
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+        const float top = col_max(m[h]);
+        const float f = __builtin_amdgcn_exp2f(m[h] - (top == -INFINITY ? 0.0f : top));
+        float sum = l[h] * f;  // of this lane's key: 16 / KEYS lanes have the same
+        sum += dpp<XOR1>(sum);
+        sum += dpp<XOR2>(sum);
+        sum += dpp<ROR4>(sum);
+        sum += dpp<ROR8>(sum);
+        sum = col_sum(sum) * (KEYS / 16.0f);
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) acc[h][j] = col_sum(acc[h][j] * f);
+        if (h < cols && g == 0) {
+            if (c == 0) {
+                part_ml[wave][0][h] = top;
+                part_ml[wave][1][h] = sum;
+            }
+#pragma unroll
+            for (int j = 0; j < DPL; ++j)
+                part_o[(wave * cols + h) * HS + row_at<T, HS>(c, j)] = acc[h][j];
+        }
+    }
+    merge_waves<float, HS, WAVES>(a, part, slot, head0, cols);
+}
+
+// Joins the parts of split requests: one workgroup a request and head. The
+// request's number of parts is not known before its lens are, so the launch
+// covers all; a request of one part is done already.
+constexpr int JOIN_THREADS = 256;
 template <typename TQ, int HS>
-__global__ __launch_bounds__(THREADS) void join_kernel(AttendArgs a) {
-    constexpr int LANES = HS / 4, SHARES = THREADS / LANES;
+__global__ __launch_bounds__(JOIN_THREADS) void join_kernel(AttendArgs a) {
+    constexpr int LANES = HS / 4, SHARES = JOIN_THREADS / LANES;
     __shared__ float4 acc_s[SHARES][LANES];
-    __shared__ float sum_s[SHARES];
-    const int r = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-    const int row = row_of(a, r);
-    if (row < 0) return;
+    __shared__ float sum_s[SHARES], top_s[SHARES];
+    const int r = blockIdx.x / a.heads, head = blockIdx.x % a.heads, tid = threadIdx.x;
+    const int row = row_of(a, r), len = len_of(a, r);
     const int2 parts = a.parts[r];
-    if (parts.y < 2) return;
-    const int d = threadIdx.x % LANES, share = threadIdx.x / LANES;
+    if ((row < 0) | (len <= UNIT) | (parts.y < 2)) return;  // (one wait for the three loads)
+    const int d = tid % LANES, share = tid / LANES;
     const long long at = (long long)parts.x * a.heads + head;
-    float top = -INFINITY;
-    for (int i = 0; i < parts.y; ++i) top = fmaxf(top, a.part_ml[at + (long long)i * a.heads].x);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    const float2 *ml = a.part_ml + at;
+    const float *po = a.part_o + at * HS + 4 * d;
+    float top = -INFINITY, sum = 0.0f;
     float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    const auto add = [&](float m, float l, float4 y) {
+        const float top1 = fmaxf(top, m), ref = top1 == -INFINITY ? 0.0f : top1;
+        const float f = __builtin_amdgcn_exp2f(top - ref), e = __builtin_amdgcn_exp2f(m - ref);
+        top = top1;
+        sum = sum * f + l * e;
+        acc.x = acc.x * f + y.x * e;
+        acc.y = acc.y * f + y.y * e;
+        acc.z = acc.z * f + y.z * e;
+        acc.w = acc.w * f + y.w * e;
+    };
+#pragma unroll 4
     for (int i = share; i < parts.y; i += SHARES) {
-        const long long s = at + (long long)i * a.heads;
-        const float2 ml = a.part_ml[s];
-        const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-        const float4 x = ld4(a.part_o + s * HS + 4 * d);
-        sum += f * ml.y;
-        acc.x += f * x.x;
-        acc.y += f * x.y;
-        acc.z += f * x.z;
-        acc.w += f * x.w;
+        const long long s = (long long)i * a.heads;
+        const float2 x = ml[s];
+        add(x.x, x.y, ld4(po + s * HS));
     }
     acc_s[share][d] = acc;
-    if (d == 0) sum_s[share] = sum;
+    if (d == 0) {
+        sum_s[share] = sum;
+        top_s[share] = top;
+    }
     __syncthreads();
     if (share != 0) return;
-    for (int i = 1; i < SHARES; ++i) {
-        sum += sum_s[i];
-        acc.x += acc_s[i][d].x;
-        acc.y += acc_s[i][d].y;
-        acc.z += acc_s[i][d].z;
-        acc.w += acc_s[i][d].w;
-    }
+#pragma unroll
+    for (int i = 1; i < SHARES; ++i) add(top_s[i], sum_s[i], acc_s[i][d]);
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     typedef vec<TQ, 4> U __attribute__((aligned(4)));
     const vec<TQ, 4> y = {(TQ)(acc.x * f), (TQ)(acc.y * f), (TQ)(acc.z * f), (TQ)(acc.w * f)};
@@ -476,24 +800,42 @@ __global__ __launch_bounds__(THREADS) void join_kernel(AttendArgs a) {
 
 // How a call is split, from what the host knows of it.
 struct Split {
-    int slots, workers;
+    int slots, workers, few, least, enough, cached;
     size_t ml_at, parts_at, bytes;  // offsets of the workspace's pieces; its size
 };
 
-constexpr int CUS = 256, WORKGROUPS_PER_CU = 4;
-constexpr int WHOLE = 256;  // sequences up to this stay whole
+constexpr int CUS = 256, WORKGROUPS_PER_CU = 8;
+constexpr long long WHOLE_FEW = 256 << 10, WHOLE_MANY = 512 << 10;
+constexpr int MANY = 96;
+constexpr long long CACHES = 120000000;
+
+// Query heads of one kv head that a workgroup takes, and workgroups they need.
+constexpr int ROWS = 4;  // up to this many, fp32 queries go by attend_rows_kernel
+int tiles_of(const PagedCache &c, const PagedBatch &b) {
+    const int group = b.heads / c.kv_heads;
+    return (group + COLS - 1) / COLS;
+}
 
 Split split_of(const PagedCache &c, const PagedBatch &b) {
-    Split s = {b.requests, 0, 0, 0, 0};
-    const long long group = b.heads / c.kv_heads, tiles = (group + COLS - 1) / COLS;
-    const long long rows = c.kv_heads * tiles;  // workgroups of one slot
-    if (b.max_len > WHOLE) {
+    Split s = {b.requests, 0, 0, 0, 0, 0, 0, 0, 0};
+    const long long rows = c.kv_heads * tiles_of(c, b);  // workgroups of one slot
+    const long long key_bytes = 2ll * c.head_size * element_size(c.type);
+    // (A whole sequence does not look at the others' lengths: half of the most they can be.)
+    s.cached = b.requests * (long long)b.max_len * key_bytes * c.kv_heads < 2 * CACHES;
+    const long long whole = b.requests * rows >= MANY ? WHOLE_MANY : WHOLE_FEW;
+    if (b.max_len * key_bytes > whole) {
         long long workers = CUS * WORKGROUPS_PER_CU / rows;
         workers = workers < 1 ? 1 : workers;
         const long long units = (b.max_len + UNIT - 1) / UNIT;
         const long long most = b.requests * units;
         workers = workers < most ? workers : most;
         s.workers = (int)workers;
+        s.cached = (int)(CACHES / (key_bytes * c.kv_heads * UNIT));
+        s.cached = s.cached < 1 ? 1 : s.cached;
+        s.few = CUS / rows < 1 ? 1 : (int)(CUS / rows);
+        const int least = (int)((64 << 10) / (key_bytes * UNIT));
+        s.least = least < 1 ? 1 : least;
+        s.enough = 4 * s.least;
         const long long slots = b.requests + workers < most ? b.requests + workers : most;
         s.slots = (int)slots;
         const size_t o = (size_t)s.slots * b.heads * c.head_size * sizeof(float);
@@ -526,26 +868,62 @@ const char *batch_fault(const PagedCache *c, const PagedBatch *b) {
     return nullptr;
 }
 
-template <template <typename, int> class POLICY, typename TC, int HS>
-void launch_attend(const AttendArgs &a, hipStream_t stream) {
-    using TQ = typename POLICY<TC, HS>::Q;
-    const dim3 grid((unsigned)((a.slots + 7) / 8 * 8 * a.kv_heads * a.tiles)), block(THREADS);
-    if (a.page.d % 16 == 0)
-        launch(attend_kernel<POLICY, TC, HS, true>, grid, block, 0, stream, a);
-    else
-        launch(attend_kernel<POLICY, TC, HS, false>, grid, block, 0, stream, a);
-    if (a.workers)
-        launch(join_kernel<TQ, HS>, dim3((unsigned)(a.requests * a.heads)), block, 0, stream, a);
+// One launch of `kernel`, whose workgroups of `waves` waves take `cols` heads each.
+void launch_parts(void (*kernel)(AttendArgs), int waves, int cols, int hs, const AttendArgs &a,
+                  hipStream_t stream) {
+    const dim3 grid((unsigned)((a.slots + 7) / 8 * 8 * a.kv_heads * a.tiles)), block(waves * WAVE);
+    const size_t lds = merge_bytes(waves, a.group < cols ? a.group : cols, hs);
+    allow_smem(kernel, lds);
+    launch(kernel, grid, block, lds, stream, a);
 }
 
-template <template <typename, int> class POLICY, typename TC>
+template <template <typename, int> class POLICY, typename TC, int HS>
+void launch_matrix(const AttendArgs &a, hipStream_t stream) {
+    launch_parts(a.page.d % 16 == 0 ? attend_kernel<POLICY, TC, HS, true>
+                                    : attend_kernel<POLICY, TC, HS, false>,
+                 4, COLS, HS, a, stream);
+}
+
+template <typename TC, int HS, int G>
+void launch_rows(const AttendArgs &a, hipStream_t stream) {
+    const bool aligned = a.page.d % 16 == 0;
+    if (a.workers == 0 && a.requests * a.kv_heads * a.tiles < 512)
+        launch_parts(aligned ? attend_rows_kernel<TC, HS, G, true, 8>
+                             : attend_rows_kernel<TC, HS, G, false, 8>,
+                     8, G, HS, a, stream);
+    else
+        launch_parts(aligned ? attend_rows_kernel<TC, HS, G, true, 4>
+                             : attend_rows_kernel<TC, HS, G, false, 4>,
+                     4, G, HS, a, stream);
+}
+
+template <typename TQ, typename TC, int HS>
+void launch_attend(const AttendArgs &a, hipStream_t stream) {
+    if constexpr (sizeof(TQ) == 2) {
+        launch_matrix<Half, TC, HS>(a, stream);
+    } else {
+        if (a.group == 1)
+            launch_rows<TC, HS, 1>(a, stream);
+        else if (a.group == 2)
+            launch_rows<TC, HS, 2>(a, stream);
+        else if (a.group <= ROWS)
+            launch_rows<TC, HS, 4>(a, stream);
+        else
+            launch_matrix<Full, TC, HS>(a, stream);
+    }
+    if (a.workers)
+        launch(join_kernel<TQ, HS>, dim3((unsigned)(a.requests * a.heads)), dim3(JOIN_THREADS), 0,
+               stream, a);
+}
+
+template <typename TQ, typename TC>
 void launch_attend(int hs, const AttendArgs &a, hipStream_t stream) {
     if (hs == 32)
-        launch_attend<POLICY, TC, 32>(a, stream);
+        launch_attend<TQ, TC, 32>(a, stream);
     else if (hs == 64)
-        launch_attend<POLICY, TC, 64>(a, stream);
+        launch_attend<TQ, TC, 64>(a, stream);
     else
-        launch_attend<POLICY, TC, 128>(a, stream);
+        launch_attend<TQ, TC, 128>(a, stream);
 }
 
 }  // namespace
@@ -566,6 +944,11 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
     if (!out || !q || !b->block_table || !b->lens) return refuse(me, "a null pointer");
     if (((uintptr_t)q | (uintptr_t)out) % 4 != 0)
         return refuse(me, "rows are no multiples of 4 bytes");
+    const int size = element_size(c->type);
+    if (c->page_size % 16 != 0 &&
+        ((c->pages - 1) * c->page_stride + (c->page_size - 1) * c->token_stride) * size / 16 >=
+            0xffffffffll)
+        return refuse(me, "a cache of 64 GiB or more needs pages of a multiple of 16 tokens");
     const Split s = split_of(*c, *b);
     char *work = (char *)b->work;
     if (work != nullptr && b->work_bytes < s.bytes) return refuse(me, "the workspace is too small");
@@ -573,29 +956,31 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
     const bool lease = s.bytes > 0 && work == nullptr;
     if (lease && stream_capturing(stream))
         return refuse(me, "a call under graph capture needs a workspace of its caller's");
-    ScratchLease ws(SCRATCH_PAGED, lease ? s.bytes : 0, stream);
+    std::optional<ScratchLease> ws;
     if (lease) {
-        if (!ws) return refuse(me, "cannot allocate the workspace");
-        work = (char *)ws.get();
+        ws.emplace(SCRATCH_PAGED, s.bytes, stream);
+        if (!*ws) return refuse(me, "cannot allocate the workspace");
+        work = (char *)ws->get();
     }
     const int group = b->heads / c->kv_heads;
     AttendArgs a = {(const char *)q, (const char *)c->k, (const char *)c->v, (char *)out, lse,
                     b->block_table, b->lens, b->rows, (float *)work, (float2 *)(work + s.ml_at),
                     (int2 *)(work + s.parts_at), c->page_stride, c->token_stride, c->head_stride,
                     b->q_stride, b->out_stride, b->requests, b->heads, c->kv_heads, group,
-                    (group + COLS - 1) / COLS, c->pages, b->table_stride, b->max_len, b->n_rows,
-                    s.slots, s.workers, b->scale * LOG2E, FastDiv::of(c->page_size)};
+                    tiles_of(*c, *b), c->pages, b->table_stride, b->max_len, b->n_rows,
+                    s.slots, s.workers, s.few, s.least, s.enough, s.cached, b->scale * LOG2E, FastDiv::of(c->page_size),
+                    (uint32_t)(c->page_stride * size / 16), (uint32_t)(c->token_stride * size / 16)};
     const int hs = c->head_size;
     if (b->type == BMB_F16)
-        launch_attend<Half, _Float16>(hs, a, stream);
+        launch_attend<_Float16, _Float16>(hs, a, stream);
     else if (b->type == BMB_BF16)
-        launch_attend<Half, __bf16>(hs, a, stream);
+        launch_attend<__bf16, __bf16>(hs, a, stream);
     else if (c->type == BMB_F16)
-        launch_attend<Full, _Float16>(hs, a, stream);
+        launch_attend<float, _Float16>(hs, a, stream);
     else if (c->type == BMB_BF16)
-        launch_attend<Full, __bf16>(hs, a, stream);
+        launch_attend<float, __bf16>(hs, a, stream);
     else
-        launch_attend<Full, float>(hs, a, stream);
+        launch_attend<float, float>(hs, a, stream);
     return 0;
 }
 

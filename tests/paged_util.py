@@ -44,10 +44,10 @@ class Problem:
         junk = torch.where(torch.rand(shape, generator=g) < 0.5, math.nan, math.inf)
         self.k, self.v = junk.to(DTYPES[cache]), junk.neg().to(DTYPES[cache])
         for r, n in enumerate(self.lens):
-            for t in range(n):
-                p = int(self.table[r, t // page])
-                self.k[p, t % page] = torch.randn(kv, hs, generator=g).to(DTYPES[cache])
-                self.v[p, t % page] = torch.randn(kv, hs, generator=g).to(DTYPES[cache])
+            t = torch.arange(n)
+            at = (self.table[r].long()[t // page], t % page)
+            self.k[at] = torch.randn(n, kv, hs, generator=g).to(DTYPES[cache])
+            self.v[at] = torch.randn(n, kv, hs, generator=g).to(DTYPES[cache])
         self.n_rows = R
         self.rows = rows
         if rows is not None:

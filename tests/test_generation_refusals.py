@@ -121,6 +121,11 @@ def test_attention_refuses_buffers(capfd):
     refused(capfd, "own type", bmb.paged_attention, c, batch(type=bmb.F16), P, P, P)
 
 
+def test_attention_refuses_huge_caches_of_odd_pages(capfd):
+    c = cache(pages=1 << 22, page_size=24, page_stride=1 << 13, token_stride=256)
+    refused(capfd, "64 GiB", bmb.paged_attention, c, batch(table_stride=64), P, P, P)
+
+
 def test_attention_refuses_small_workspaces(capfd):
     b = batch(max_len=64000, table_stride=4000)
     need = bmb.paged_attention_workspace(cache(), b)

@@ -176,9 +176,9 @@ def test_attention_edges(gpu, type, cache, hs, heads, kv, page, layout):
 
 @pytest.mark.parametrize("type,cache", TYPES)
 @pytest.mark.parametrize("hs", [32, 64, 128])
-@pytest.mark.parametrize("lens,heads,kv,page", [([1500], 12, 12, 16), ([257, 0, 1, 900], 8, 2, 24),
-                                                ([3000, 2], 20, 1, 32),
-                                                ([300] * 70 + [0, 1, 2500], 2, 2, 16)])
+@pytest.mark.parametrize("lens,heads,kv,page", [([4500], 12, 12, 16), ([257, 0, 1, 2500], 8, 2, 24),
+                                                ([3000, 2], 20, 1, 32), ([2600, 129], 3, 1, 48),
+                                                ([300] * 70 + [0, 1, 5000], 2, 2, 16)])
 def test_attention_split(gpu, type, cache, hs, lens, heads, kv, page):
     print("attention split", type, cache, hs, lens[:4], heads, kv, page, flush=True)
     p = Problem(lens, heads, kv, hs, type, cache, page, "head", seed=hs).device()
@@ -280,9 +280,10 @@ def test_attention_interleaved_halves_and_null_lse(gpu):
     d.check()
 
 
-def test_attention_offsets_past_32_bits(gpu):
+@pytest.mark.parametrize("page", [16, 12])
+def test_attention_offsets_past_32_bits(gpu, page):
     """Pages whose places lie more than 2^32 elements into the buffer."""
-    kv, hs, page = 8, 128, 16
+    kv, hs = 8, 128
     pages = (1 << 32) // (page * kv * hs) + 8
     k = torch.zeros(pages, page, kv, hs, dtype=torch.float16, device="cuda")
     v = torch.zeros_like(k)
@@ -333,7 +334,7 @@ def test_attention_streams_and_scratch(gpu):
 def test_attention_captured(gpu):
     """Captured with a workspace, replayed with other lengths and queries each
     time; without one the capture is refused before anything is queued."""
-    lens = [600, 3, 900]
+    lens = [600, 3, 1400]
     d = Problem(lens, 8, 2, 64, "bf16", "bf16", 16, seed=12).device()
     d.workspace()
     side = torch.cuda.Stream()
@@ -347,7 +348,7 @@ def test_attention_captured(gpu):
             d.run(side.cuda_stream)
         d.batch.work = work
     other = Problem([50, 60], 4, 4, 64, "f32", "f32", 16, seed=13).device()
-    for now in ([600, 3, 900], [599, 0, 17], [1, 2, 899]):
+    for now in ([600, 3, 1400], [599, 0, 17], [1, 2, 1399]):
         d.p.lens = now
         d.lens.copy_(ints(now))
         d.out.fill_(768.0)
