@@ -7,8 +7,7 @@
 namespace bmb {
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
-constexpr int PLAN_MAX_REQUESTS = 8192;  // 12 bytes of LDS each
+constexpr int PLAN_MAX_REQUESTS = 8192;  // 16 bytes of LDS each
 constexpr int PLAN_MAX_BLOCKS = 512;
 
 struct PlanArgs {
@@ -30,17 +29,17 @@ __device__ __forceinline__ Ask ask_of(const PlanArgs &a, int r) {
     Ask x;
     const int n = p.new_tokens[r];
     x.held = min(max(p.lens[r], 0), cap);
-    x.have = a.page.quot(x.held) + (a.page.quot(x.held) * p.page_size < x.held);
+    x.have = a.page.quot(x.held + p.page_size - 1);
     x.ended = n < 0;
     x.want = n > 0 && n <= cap - x.held ? n : 0;
-    const int upto = x.held + (int)x.want, q = a.page.quot(upto);
-    x.need = x.want ? q + (q * p.page_size < upto) - x.have : 0;
+    x.need = x.want ? a.page.quot(x.held + (int)x.want + p.page_size - 1) - x.have : 0;
     return x;
 }
 
 // Inclusive scans of two counts over the workgroup; totals are their last
 // values. A wave sums its rows of 64 in registers, then every wave adds the
 // sums of the waves before it.
+template <int THREADS>
 __device__ __forceinline__ void block_scan(uint32_t &x, uint32_t &y, uint32_t &tx, uint32_t &ty,
                                            uint32_t (*part)[2]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -55,7 +54,7 @@ __device__ __forceinline__ void block_scan(uint32_t &x, uint32_t &y, uint32_t &t
     uint32_t bx = 0, by = 0;
     tx = ty = 0;
 #pragma unroll
-    for (int w = 0; w < PLAN_THREADS / WAVE; ++w) {
+    for (int w = 0; w < THREADS / WAVE; ++w) {
         if (w == wave) {
             bx = tx;
             by = ty;
@@ -76,15 +75,17 @@ __device__ __forceinline__ void block_scan(uint32_t &x, uint32_t &y, uint32_t &t
 // Only lens and state may be the caller's outputs too (in place): then those
 // are written by a launch of their own, or, with one workgroup, behind a
 // barrier.
-__global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(PlanArgs a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void plan_kernel(PlanArgs a) {
     extern __shared__ uint32_t plan_lds[];
-    __shared__ uint32_t part[PLAN_THREADS / WAVE][2];
+    __shared__ uint32_t part[THREADS / WAVE][2];
     __shared__ uint32_t n_gone, taken, limit;
     const PagedPlan &p = a.p;
     const int R = p.requests, tid = threadIdx.x;
     uint32_t *off = plan_lds;          // R + 1: tokens before a request
     uint32_t *first = off + R + 1;     // R: pages taken (given back) before it
-    uint32_t *gone = first + R;        // ended requests this workgroup handles
+    uint32_t *held = first + R;        // R: tokens held
+    uint32_t *gone = held + R;         // ended requests this workgroup handles
     const uint32_t pages = p.pages;
     const uint32_t head = (uint32_t)p.state[0] % pages;
     const uint32_t count = min((uint32_t)max(p.state[1], 0), pages);
@@ -95,19 +96,19 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(PlanArgs a) {
         off[0] = 0;
     }
     uint32_t asked = 0, back = 0, tokens_asked = 0;
-    for (int base = 0; base < R; base += PLAN_THREADS) {
+    for (int base = 0; base < R; base += THREADS) {
         const int r = base + tid;
         Ask x = {0, 0, 0u, 0u, false};
         if (r < R) x = ask_of(a, r);
         uint32_t pages_upto = x.need, back_upto = x.ended ? x.have : 0, t0, t1;
-        block_scan(pages_upto, back_upto, t0, t1, part);
+        block_scan<THREADS>(pages_upto, back_upto, t0, t1, part);
         pages_upto = add_sat(asked, pages_upto);
         back_upto = add_sat(back, back_upto);
         asked = add_sat(asked, t0);
         back = add_sat(back, t1);
         const bool has_pages = x.want > 0 && (x.need == 0 || pages_upto <= count);
         uint32_t tok = has_pages ? x.want : 0, none = 0;
-        block_scan(tok, none, t0, t1, part);
+        block_scan<THREADS>(tok, none, t0, t1, part);
         tok = add_sat(tokens_asked, tok);
         tokens_asked = add_sat(tokens_asked, t0);
         // The granted requests are those before the first that would pass
@@ -118,37 +119,36 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(PlanArgs a) {
         if (ok && x.need > 0) atomicMax(&taken, pages_upto);
         if (r < R) {
             off[r + 1] = tok;
+            held[r] = x.held;
             first[r] = x.ended ? back_upto - x.have : pages_upto - x.need;
             if (x.ended && x.have > 0 && r % gridDim.x == blockIdx.x)
                 gone[atomicAdd(&n_gone, 1u)] = r;
         }
     }
     __syncthreads();
-    for (int r = tid; r < R; r += PLAN_THREADS) off[r + 1] = min(off[r + 1], limit);
+    for (int r = tid; r < R; r += THREADS) off[r + 1] = min(off[r + 1], limit);
     __syncthreads();
 
     if (a.fill) {
         const uint32_t T = p.max_tokens, tokens = off[R];
-        for (uint32_t t = blockIdx.x * PLAN_THREADS + tid; t < T; t += gridDim.x * PLAN_THREADS) {
+        for (uint32_t t = blockIdx.x * THREADS + tid; t < T; t += gridDim.x * THREADS) {
             int slot = -1, pos = 0;
             if (t < tokens) {
-                int lo = 0, hi = R - 1;  // the last request with off <= t that has tokens
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
+                int r = 0, hi = R - 1;  // t's request: the first that ends behind it
+                while (r < hi) {
+                    const int mid = (r + hi) >> 1;
                     if (off[mid + 1] <= t)
-                        lo = mid + 1;
+                        r = mid + 1;
                     else
                         hi = mid;
                 }
-                const int held = min(max(p.lens[lo], 0), p.max_pages * p.page_size);
-                const int q = a.page.quot(held), have = q + (q * p.page_size < held);
-                pos = held + (int)(t - off[lo]);
+                const int have = a.page.quot(held[r] + p.page_size - 1);
+                pos = (int)(held[r] + (t - off[r]));
                 const int j = a.page.quot(pos), in = pos - j * p.page_size;
-                int *row = p.block_table + (size_t)lo * p.max_pages;
+                int *row = p.block_table + (size_t)r * p.max_pages;
                 int page;
                 if (j >= have) {
-                    const uint32_t at = (head + first[lo] + (uint32_t)(j - have)) % pages;
-                    page = p.free_pages[at];
+                    page = p.free_pages[(head + first[r] + (uint32_t)(j - have)) % pages];
                     if (in == 0) row[j] = page;
                 } else {
                     page = row[j];
@@ -158,22 +158,19 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(PlanArgs a) {
             p.slots[t] = slot;
             p.positions[t] = pos;
         }
-        for (uint32_t i = tid >> 6; i < n_gone; i += PLAN_THREADS / WAVE) {
-            const int r = gone[i];
-            const int held = min(max(p.lens[r], 0), p.max_pages * p.page_size);
-            const int q = a.page.quot(held), have = q + (q * p.page_size < held);
+        for (uint32_t i = tid >> 6; i < n_gone; i += THREADS / WAVE) {
+            const int r = gone[i], have = a.page.quot(held[r] + p.page_size - 1);
             const int *row = p.block_table + (size_t)r * p.max_pages;
-            for (int j = tid & 63; j < have; j += WAVE)
-                p.free_pages[(head + count + first[r] + (uint32_t)j) % pages] = row[j];
+            const uint32_t to = head + count + first[r];
+            for (int j = tid & 63; j < have; j += WAVE) p.free_pages[(to + (uint32_t)j) % pages] = row[j];
         }
     }
     if (a.finish && blockIdx.x == 0) {
         __syncthreads();  // lens and state may be the results too
-        for (int r = tid; r < R; r += PLAN_THREADS) {
+        for (int r = tid; r < R; r += THREADS) {
             const uint32_t grant = off[r + 1] - off[r];
-            const int held = min(max(p.lens[r], 0), p.max_pages * p.page_size);
             const bool ended = p.new_tokens[r] < 0;
-            p.lens_out[r] = ended ? 0 : held + (int)grant;
+            p.lens_out[r] = ended ? 0 : (int)(held[r] + grant);
             p.rows[r] = grant ? (int)off[r + 1] - 1 : -1;
             p.offsets[r + 1] = off[r + 1];
         }
@@ -247,7 +244,7 @@ int paged_plan(const PagedPlan *p, hipStream_t stream) {
     if (p->max_pages < 1 || p->pages < 1 || p->page_size < 1 || p->max_tokens < 0)
         return refuse(me, "a size is below its least");
     if ((long long)p->pages * p->page_size > INT_MAX ||
-        (long long)p->max_pages * p->page_size > INT_MAX)
+        ((long long)p->max_pages + 1) * p->page_size > INT_MAX)
         return refuse(me, "2^31 or more tokens in the cache or in a request");
     if (!p->new_tokens || !p->lens || !p->lens_out || !p->state || !p->state_out ||
         !p->free_pages || !p->block_table || !p->rows || !p->offsets ||
@@ -262,16 +259,24 @@ int paged_plan(const PagedPlan *p, hipStream_t stream) {
         return refuse(me, "lens or state overlaps its result in part");
     const bool in_place = p->lens == p->lens_out || p->state == p->state_out;
     PlanArgs a = {*p, FastDiv::of(p->page_size), true, true};
-    const size_t lds = (3 * R + 1) * sizeof(uint32_t);
-    allow_smem(plan_kernel, lds + 256);
-    int blocks = (p->max_tokens + PLAN_THREADS - 1) / PLAN_THREADS;
+    // As many waves as one round of the scan needs: 64 decoding requests take
+    // 4.8 us with 64 threads (their tables and ended requests then go one by
+    // one), 4.1 with 256, 4.7 with 1024; 8 requests 3.2, 3.5 and 4.2; 1024
+    // requests 18.6, 9.0 and 6.6.
+    const int threads = R <= 32 ? 64 : R <= 256 ? 256 : 1024;
+    const auto kernel = threads == 64    ? plan_kernel<64>
+                        : threads == 256 ? plan_kernel<256>
+                                         : plan_kernel<1024>;
+    const size_t lds = (4 * R + 1) * sizeof(uint32_t);
+    allow_smem(kernel, lds + 256);
+    int blocks = (int)(((long long)p->max_tokens + threads - 1) / threads);
     blocks = blocks < 1 ? 1 : blocks > PLAN_MAX_BLOCKS ? PLAN_MAX_BLOCKS : blocks;
     a.finish = blocks == 1 || !in_place;
-    launch(plan_kernel, dim3(blocks), dim3(PLAN_THREADS), lds, stream, a);
+    launch(kernel, dim3(blocks), dim3(threads), lds, stream, a);
     if (!a.finish) {
         a.fill = false;
         a.finish = true;
-        launch(plan_kernel, dim3(1), dim3(PLAN_THREADS), lds, stream, a);
+        launch(kernel, dim3(1), dim3(threads), lds, stream, a);
     }
     return 0;
 }

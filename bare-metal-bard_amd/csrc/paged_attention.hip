@@ -30,7 +30,6 @@
 namespace bmb {
 namespace {
 
-constexpr int COLS = 16;
 constexpr int UNIT = 128;  // a part is a whole number of these keys
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -79,7 +78,7 @@ __device__ __forceinline__ int len_of(const AttendArgs &a, int r) {
 // its slot's request by itself, 64 requests at a time.
 __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
-    Part p = {slot, 0, 0, 0, 0, -1, a.cached == 0};
+    Part p = {slot, 0, 0, 0, 0, -1, a.cached == 0 && a.tiles == 1};
     if (a.workers == 0) {
         p.row = row_of(a, slot);
         p.n = p.row >= 0;
@@ -93,7 +92,7 @@ __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
         if (r < a.requests && row_of(a, r) >= 0) units = (len_of(a, r) + UNIT - 1) / UNIT;
         total += __builtin_amdgcn_readlane(wave_scan(units), 63);
     }
-    p.nt = total >= (uint32_t)a.cached;
+    p.nt = total >= (uint32_t)a.cached && a.tiles == 1;  // (several tiles read the same rows)
     uint32_t size = (total + a.workers - 1) / a.workers;
     size = max(size, min((total + a.few - 1) / a.few, (uint32_t)a.enough));
     size = max(size, (uint32_t)a.least);
@@ -362,14 +361,14 @@ __device__ __forceinline__ unsigned load_step(typename P::Regs &x, const AttendA
 }
 
 // LDS of a workgroup: each wave's running maxima and sums, and its share of
-// the result for the columns in use.
-constexpr size_t merge_bytes(int waves, int cols, int hs) {
-    return (size_t)waves * (2 * COLS + cols * hs) * sizeof(float);
+// the result for the columns in use, `used` of `cols`.
+constexpr size_t merge_bytes(int waves, int cols, int used, int hs) {
+    return (size_t)waves * (2 * cols + used * hs) * sizeof(float);
 }
 
 // The waves' results, each weighed by its maximum: to the result, or as a part
 // of a split request.
-template <typename TQ, int HS, int WAVES>
+template <typename TQ, int HS, int WAVES, int COLS>
 __device__ __forceinline__ void merge_waves(const AttendArgs &a, const Part &part, int slot,
                                             int head0, int cols) {
     extern __shared__ float merge[];
@@ -406,11 +405,12 @@ __device__ __forceinline__ void merge_waves(const AttendArgs &a, const Part &par
         a.parts[part.r] = make_int2(slot, part.n);
 }
 
-// A wave's share of a part: steps of keys from `first` on, `step` apart.
-template <typename P, bool ALIGNED, bool NT>
-__device__ __forceinline__ void attend_steps(f32x4 (&o)[P::DPL], float &m, float &l,
+// A wave's share of a part: steps of keys from `first` on, `step` apart, for QT
+// groups of 16 query heads.
+template <typename P, bool ALIGNED, bool NT, int QT>
+__device__ __forceinline__ void attend_steps(f32x4 (&o)[QT][P::DPL], float (&m)[QT], float (&l)[QT],
                                              const AttendArgs &a, const Part &part,
-                                             const typename P::Query &q, const int *table,
+                                             const typename P::Query (&q)[QT], const int *table,
                                              const char *k, const char *v, int first, int step,
                                              int g, int c) {
     constexpr int DPL = P::DPL, KV = P::KV;
@@ -421,50 +421,54 @@ __device__ __forceinline__ void attend_steps(f32x4 (&o)[P::DPL], float &m, float
         next.fetch(a, table, kb + step, part.end);
         const unsigned live = load_step<P, ALIGNED, NT>(x, a, pages, k, v, kb, part.end, g, c);
         const bool whole = __builtin_amdgcn_ballot_w64(live != (1u << KV) - 1) == 0;
-        float p[KV];
-#pragma unroll
-        for (int t = 0; t < P::TILES; ++t) {
-            const f32x4 s = P::scores(x, t, q);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[4 * t + r] = s[r] * a.scale;
-        }
         if (!whole) {
-            // What lies in an absent place may be NaN or infinite: the score
-            // and the value are replaced, not multiplied by 0.
+            // What lies in an absent place may be NaN or infinite: the value
+            // (and the score, below) is replaced, not multiplied by 0.
+#pragma unroll
+            for (int i = 0; i < KV; ++i)
+                if (!(live >> i & 1)) P::zero_v(x, i);
+        }
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            float p[KV];
+#pragma unroll
+            for (int t = 0; t < P::TILES; ++t) {
+                const f32x4 s = P::scores(x, t, q[u]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[4 * t + r] = s[r] * a.scale;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < KV; ++i) p[i] = live >> i & 1 ? p[i] : -INFINITY;
+            }
+            float top = p[0];
+#pragma unroll
+            for (int i = 1; i < KV; ++i) top = fmaxf(top, p[i]);
+            const float m1 = fmaxf(m[u], col_max(top));
+            const float ref = m1 == -INFINITY ? 0.0f : m1;  // no live score yet: all 2^-inf
+            const float keep = __builtin_amdgcn_exp2f(m[u] - ref);
+            m[u] = m1;
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < KV; ++i) {
-                const bool on = live >> i & 1;
-                p[i] = on ? p[i] : -INFINITY;
-                if (!on) P::zero_v(x, i);
+                p[i] = __builtin_amdgcn_exp2f(p[i] - ref);
+                sum += p[i];
             }
+            l[u] = l[u] * keep + sum;
+#pragma unroll
+            for (int j = 0; j < DPL; ++j) o[u][j] *= keep;
+            P::values(o[u], x, p);
         }
-        float top = p[0];
-#pragma unroll
-        for (int i = 1; i < KV; ++i) top = fmaxf(top, p[i]);
-        const float m1 = fmaxf(m, col_max(top));
-        const float ref = m1 == -INFINITY ? 0.0f : m1;  // no live score yet: all 2^-inf
-        const float keep = __builtin_amdgcn_exp2f(m - ref);
-        m = m1;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < KV; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(p[i] - ref);
-            sum += p[i];
-        }
-        l = l * keep + sum;
-#pragma unroll
-        for (int j = 0; j < DPL; ++j) o[j] *= keep;
-        P::values(o, x, p);
     }
 }
 
-template <template <typename, int> class POLICY, typename TC, int HS, bool ALIGNED>
+template <template <typename, int> class POLICY, typename TC, int HS, bool ALIGNED, int QT>
 __global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
     using P = POLICY<TC, HS>;
     using TQ = typename P::Q;
-    constexpr int WAVES = 4, STEP = 16 * P::TILES, DPL = P::DPL;
+    constexpr int WAVES = 4, STEP = 16 * P::TILES, DPL = P::DPL, COLS = 16 * QT;
     extern __shared__ float merge[];
-    float(*part_ml)[2][COLS] = (float(*)[2][COLS])merge;
+    float *part_ml = merge;                     // (wave, maximum and sum, column)
     float *part_o = merge + WAVES * 2 * COLS;  // (wave, column, element)
 
     // Workgroups go to the XCDs in turn: all heads of a slot on one of them,
@@ -484,35 +488,44 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
     const char *k = a.k + kv_head * a.head_stride * (long long)sizeof(TC);
     const char *v = a.v + kv_head * a.head_stride * (long long)sizeof(TC);
 
-    typename P::Query q;
-    if (c < cols)
-        P::load_q(q, (const TQ *)a.q + part.row * a.q_stride + (head0 + c) * HS, g);
-    else
-        P::zero_q(q);
-
-    f32x4 o[DPL];
+    typename P::Query q[QT];
+    f32x4 o[QT][DPL];
+    float m[QT], l[QT];  // of column c; l of this lane's keys only
 #pragma unroll
-    for (int j = 0; j < DPL; ++j) o[j] = {0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;  // of column c; l of this lane's keys only
+    for (int u = 0; u < QT; ++u) {
+        const int col = 16 * u + c;
+        if (col < cols)
+            P::load_q(q[u], (const TQ *)a.q + part.row * a.q_stride + (head0 + col) * HS, g);
+        else
+            P::zero_q(q[u]);
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) o[u][j] = {0.0f, 0.0f, 0.0f, 0.0f};
+        m[u] = -INFINITY;
+        l[u] = 0.0f;
+    }
     if (part.nt)
-        attend_steps<P, ALIGNED, true>(o, m, l, a, part, q, table, k, v, wave * STEP, WAVES * STEP, g, c);
+        attend_steps<P, ALIGNED, true, QT>(o, m, l, a, part, q, table, k, v, wave * STEP,
+                                           WAVES * STEP, g, c);
     else
-        attend_steps<P, ALIGNED, false>(o, m, l, a, part, q, table, k, v, wave * STEP, WAVES * STEP, g, c);
-    l = col_sum(l);
-
-    // The waves' results through LDS, each weighed by its maximum.
-    if (g == 0) {
-        part_ml[wave][0][c] = m;
-        part_ml[wave][1][c] = l;
-    }
-    if (c < cols) {
+        attend_steps<P, ALIGNED, false, QT>(o, m, l, a, part, q, table, k, v, wave * STEP,
+                                            WAVES * STEP, g, c);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+    for (int u = 0; u < QT; ++u) {
+        const int col = 16 * u + c;
+        const float sum = col_sum(l[u]);
+        if (g == 0) {
+            part_ml[(wave * 2 + 0) * COLS + col] = m[u];
+            part_ml[(wave * 2 + 1) * COLS + col] = sum;
+        }
+        if (col < cols) {
 #pragma unroll
-            for (int j = 0; j < DPL; ++j)
-                part_o[(wave * cols + c) * HS + (4 * g + r) * DPL + j] = o[j][r];
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < DPL; ++j)
+                    part_o[(wave * cols + col) * HS + (4 * g + r) * DPL + j] = o[u][j][r];
+        }
     }
-    merge_waves<TQ, HS, WAVES>(a, part, slot, head0, cols);
+    merge_waves<TQ, HS, WAVES, COLS>(a, part, slot, head0, cols);
 }
 
 // ---- few query heads to a kv head, fp32 queries: 16 matrix columns would
@@ -682,8 +695,8 @@ __global__ __launch_bounds__(WAVES *WAVE) void attend_rows_kernel(AttendArgs a) 
     constexpr int KEYS = BYTES >= 32 ? 4 : BYTES == 16 ? 8 : 16;  // 32 registers each of K and V
     constexpr int STEP = 4 * KEYS;
     extern __shared__ float merge[];
-    float(*part_ml)[2][COLS] = (float(*)[2][COLS])merge;
-    float *part_o = merge + WAVES * 2 * COLS;  // (wave, head, element)
+    float(*part_ml)[2][G] = (float(*)[2][G])merge;
+    float *part_o = merge + WAVES * 2 * G;  // (wave, head, element)
 
     const int per = 8 * a.kv_heads * a.tiles;
     const int in = blockIdx.x % per, slot = blockIdx.x / per * 8 + in % 8;
@@ -742,7 +755,7 @@ __global__ __launch_bounds__(WAVES *WAVE) void attend_rows_kernel(AttendArgs a) 
                 part_o[(wave * cols + h) * HS + row_at<T, HS>(c, j)] = acc[h][j];
         }
     }
-    merge_waves<float, HS, WAVES>(a, part, slot, head0, cols);
+    merge_waves<float, HS, WAVES, G>(a, part, slot, head0, cols);
 }
 
 // Joins the parts of split requests: one workgroup a request and head. The
@@ -813,7 +826,8 @@ constexpr long long CACHES = 120000000;
 constexpr int ROWS = 4;  // up to this many, fp32 queries go by attend_rows_kernel
 int tiles_of(const PagedCache &c, const PagedBatch &b) {
     const int group = b.heads / c.kv_heads;
-    return (group + COLS - 1) / COLS;
+    const int cols = b.type != BMB_F32 && group > 16 ? 32 : 16;
+    return (group + cols - 1) / cols;
 }
 
 Split split_of(const PagedCache &c, const PagedBatch &b) {
@@ -872,16 +886,16 @@ const char *batch_fault(const PagedCache *c, const PagedBatch *b) {
 void launch_parts(void (*kernel)(AttendArgs), int waves, int cols, int hs, const AttendArgs &a,
                   hipStream_t stream) {
     const dim3 grid((unsigned)((a.slots + 7) / 8 * 8 * a.kv_heads * a.tiles)), block(waves * WAVE);
-    const size_t lds = merge_bytes(waves, a.group < cols ? a.group : cols, hs);
+    const size_t lds = merge_bytes(waves, cols, a.group < cols ? a.group : cols, hs);
     allow_smem(kernel, lds);
     launch(kernel, grid, block, lds, stream, a);
 }
 
-template <template <typename, int> class POLICY, typename TC, int HS>
+template <template <typename, int> class POLICY, typename TC, int HS, int QT>
 void launch_matrix(const AttendArgs &a, hipStream_t stream) {
-    launch_parts(a.page.d % 16 == 0 ? attend_kernel<POLICY, TC, HS, true>
-                                    : attend_kernel<POLICY, TC, HS, false>,
-                 4, COLS, HS, a, stream);
+    launch_parts(a.page.d % 16 == 0 ? attend_kernel<POLICY, TC, HS, true, QT>
+                                    : attend_kernel<POLICY, TC, HS, false, QT>,
+                 4, 16 * QT, HS, a, stream);
 }
 
 template <typename TC, int HS, int G>
@@ -900,7 +914,10 @@ void launch_rows(const AttendArgs &a, hipStream_t stream) {
 template <typename TQ, typename TC, int HS>
 void launch_attend(const AttendArgs &a, hipStream_t stream) {
     if constexpr (sizeof(TQ) == 2) {
-        launch_matrix<Half, TC, HS>(a, stream);
+        if (a.group <= 16)
+            launch_matrix<Half, TC, HS, 1>(a, stream);
+        else
+            launch_matrix<Half, TC, HS, 2>(a, stream);
     } else {
         if (a.group == 1)
             launch_rows<TC, HS, 1>(a, stream);
@@ -909,7 +926,7 @@ void launch_attend(const AttendArgs &a, hipStream_t stream) {
         else if (a.group <= ROWS)
             launch_rows<TC, HS, 4>(a, stream);
         else
-            launch_matrix<Full, TC, HS>(a, stream);
+            launch_matrix<Full, TC, HS, 1>(a, stream);
     }
     if (a.workers)
         launch(join_kernel<TQ, HS>, dim3((unsigned)(a.requests * a.heads)), dim3(JOIN_THREADS), 0,

@@ -151,7 +151,9 @@ class Case:
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,V,stride", [(1, 1, None), (5, 65, 128), (4, 4095, None), (3, 4096, 4096),
                                            (4, 4097, 4100), (6, 50257, None), (5, 50257, 50304),
-                                           (3, 12289, 12291), (70, 33, 33)])
+                                           (3, 12289, 12291), (70, 33, 33),
+                                           # results past 32 MB, and just below
+                                           (340, 50257, None), (160, 50257, 50259)])
 def test_logits(gpu, type, rows, V, stride):
     print("logits", type, rows, V, stride, flush=True)
     Case(rows, V, type, stride, seed=V).run()

@@ -166,7 +166,7 @@ def test_append(gpu, type, cache, tokens, kv, hs, page, layout):
 @pytest.mark.parametrize("hs", [32, 64, 128])
 @pytest.mark.parametrize("heads,kv,page,layout", [(3, 3, 16, "token"), (8, 2, 16, "head"),
                                                   (5, 1, 7, "token"), (34, 2, 64, "head"),
-                                                  (2, 2, 1, "head")])
+                                                  (2, 2, 1, "head"), (66, 2, 32, "token")])
 def test_attention_edges(gpu, type, cache, hs, heads, kv, page, layout):
     print("attention edges", type, cache, hs, heads, kv, page, flush=True)
     p = Problem(EDGES, heads, kv, hs, type, cache, page, layout, seed=hs + heads).device()
@@ -177,7 +177,7 @@ def test_attention_edges(gpu, type, cache, hs, heads, kv, page, layout):
 @pytest.mark.parametrize("type,cache", TYPES)
 @pytest.mark.parametrize("hs", [32, 64, 128])
 @pytest.mark.parametrize("lens,heads,kv,page", [([4500], 12, 12, 16), ([257, 0, 1, 2500], 8, 2, 24),
-                                                ([3000, 2], 20, 1, 32), ([2600, 129], 3, 1, 48),
+                                                ([3000, 2], 20, 1, 32), ([2600, 129], 3, 1, 48), ([2500, 700], 40, 1, 10),
                                                 ([300] * 70 + [0, 1, 5000], 2, 2, 16)])
 def test_attention_split(gpu, type, cache, hs, lens, heads, kv, page):
     print("attention split", type, cache, hs, lens[:4], heads, kv, page, flush=True)
