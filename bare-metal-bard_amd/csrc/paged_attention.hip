@@ -47,12 +47,12 @@ struct AttendArgs {
     int2 *parts;       // (requests): first slot, number of parts
     long long page_stride, token_stride, head_stride, q_stride, out_stride;
     int requests, heads, kv_heads, group, tiles, pages, table_stride, max_len, n_rows;
-    int slots;     // parts that the launch has room for
-    int workers;   // parts aimed at; 0: one part a request
-    int few;       // parts at one workgroup a CU
-    int least, enough;  // units of a part: at least, and no fewer parts than `few` for more
-    int cached;    // units from which on a batch passes the caches
-    float scale;   // times log2(e)
+    int slots;          // parts that the launch has room for
+    int workers;        // most parts; 0: one part a request
+    int few;            // parts that give each CU a workgroup
+    int least, enough;  // units of a part: at least; more than `enough` only past `few` parts
+    int cached;         // units that stay in the caches; without workers: whether they do
+    float scale;        // times log2(e)
     FastDiv page;
     uint32_t page16, token16;  // strides in units of 16 bytes
 };
@@ -295,36 +295,42 @@ constexpr uint32_t NO_ROW = 0xffffffffu;
 template <bool ALIGNED, int TILES>
 struct Pages {
     int id[ALIGNED ? TILES : 1];
+    // (Steps behind `end`, which is at least 1, look up the last tile or key
+    // again: a branch here would have the scalar loads waited for at once.)
+    static __device__ __forceinline__ int tile_at(int t, int kb, int end) {
+        return min(kb + 16 * t, (end - 1) & ~15);
+    }
+    static __device__ __forceinline__ int key_at(int kb) {
+        return kb + (int)(threadIdx.x & (16 * TILES - 1));
+    }
     __device__ __forceinline__ void fetch(const AttendArgs &a, const int *table, int kb, int end) {
         if constexpr (ALIGNED) {
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
-                id[t] = kb + 16 * t < end ? table[a.page.quot(kb + 16 * t)] : -1;
+            for (int t = 0; t < TILES; ++t) id[t] = table[a.page.quot(tile_at(t, kb, end))];
         } else {
-            const int key = kb + (int)(threadIdx.x & (16 * TILES - 1));
-            id[0] = key < end ? table[a.page.quot(key)] : -1;
+            id[0] = table[a.page.quot(min(key_at(kb), end - 1))];
         }
     }
     // Not ALIGNED: the place of this lane's key.
-    __device__ __forceinline__ uint32_t place(const AttendArgs &a, int kb) const {
-        const int key = kb + (int)(threadIdx.x & (16 * TILES - 1));
+    __device__ __forceinline__ uint32_t place(const AttendArgs &a, int kb, int end) const {
+        const int key = key_at(kb);
         const uint32_t in = key - a.page.quot(key) * (int)a.page.d;
-        return (unsigned)id[0] < (unsigned)a.pages ? id[0] * a.page16 + in * a.token16 : NO_ROW;
+        const bool ok = key < end && (unsigned)id[0] < (unsigned)a.pages;
+        return ok ? id[0] * a.page16 + in * a.token16 : NO_ROW;
     }
-    // ALIGNED: the place of a tile's first key, and how many of it count (none:
-    // the first rows of the cache, which are left out).
-    __device__ __forceinline__ void tile(const AttendArgs &a, int t, int kb, int end, int esize,
-                                         int &n, long long &at) const {
-        const int base = kb + 16 * t;
-        n = (unsigned)id[t] < (unsigned)a.pages ? min(end - base, 16) : 0;
-        const int in = base - a.page.quot(base) * (int)a.page.d;
-        at = n > 0 ? (id[t] * a.page_stride + in * a.token_stride) * esize : 0;
+    // ALIGNED: bytes to a tile's first key, and how many of its keys count (with
+    // none, the rows that are read all the same are some of the cache's).
+    __device__ __forceinline__ long long tile(const AttendArgs &a, int t, int kb, int end,
+                                              int esize, int &n) const {
+        const int base = tile_at(t, kb, end), in = base - a.page.quot(base) * (int)a.page.d;
+        const bool ok = (unsigned)id[t] < (unsigned)a.pages;
+        n = ok ? min(end - (kb + 16 * t), 16) : 0;
+        return ((ok ? id[t] : 0) * a.page_stride + in * a.token_stride) * esize;
     }
 };
 
 // Loads the step of keys from kb on. Returns which of the lane's KV keys (4g +
-// r of each 16) count. Keys behind `end` are read where their page goes on, or
-// from the first row, and left out.
+// r of each 16) count.
 template <typename P, bool ALIGNED, bool NT>
 __device__ __forceinline__ unsigned load_step(typename P::Regs &x, const AttendArgs &a,
                                               const Pages<ALIGNED, P::TILES> &pages,
@@ -332,13 +338,12 @@ __device__ __forceinline__ unsigned load_step(typename P::Regs &x, const AttendA
                                               int c) {
     unsigned live = 0;
     uint32_t place = 0;
-    if constexpr (!ALIGNED) place = pages.place(a, kb);
+    if constexpr (!ALIGNED) place = pages.place(a, kb, end);
 #pragma unroll
     for (int t = 0; t < P::TILES; ++t) {
         if constexpr (ALIGNED) {
             int n;
-            long long at;
-            pages.tile(a, t, kb, end, P::SIZE, n, at);
+            const long long at = pages.tile(a, t, kb, end, P::SIZE, n);
             const long long row = a.token_stride * P::SIZE;
             P::template load_k<NT>(x, t, k + at + c * row, g);
 #pragma unroll
@@ -415,6 +420,7 @@ __device__ __forceinline__ void attend_steps(f32x4 (&o)[QT][P::DPL], float (&m)[
                                              int g, int c) {
     constexpr int DPL = P::DPL, KV = P::KV;
     Pages<ALIGNED, P::TILES> pages, next;
+    if (part.begin + first >= part.end) return;
     pages.fetch(a, table, part.begin + first, part.end);
     for (int kb = part.begin + first; kb < part.end; kb += step, pages = next) {
         typename P::Regs x;
@@ -618,8 +624,7 @@ __device__ __forceinline__ unsigned load_rows(vec<T, HS / 16> (&kr)[KEYS],
 #pragma unroll
         for (int t = 0; t < KEYS / 4; ++t) {
             int n;
-            long long at;
-            pages.tile(a, t, kb, end, sizeof(T), n, at);
+            const long long at = pages.tile(a, t, kb, end, sizeof(T), n);
             const long long row = a.token_stride * (int)sizeof(T);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -630,7 +635,7 @@ __device__ __forceinline__ unsigned load_rows(vec<T, HS / 16> (&kr)[KEYS],
             }
         }
     } else {
-        const uint32_t place = pages.place(a, kb);
+        const uint32_t place = pages.place(a, kb, end);
 #pragma unroll
         for (int i = 0; i < KEYS; ++i) {
             const uint32_t at = __shfl(place, 4 * i + g);
@@ -652,6 +657,7 @@ __device__ __forceinline__ void rows_steps(float (&acc)[G][HS / 16], float (&m)[
     constexpr int DPL = HS / 16;
     using Row = vec<T, DPL>;
     Pages<ALIGNED, KEYS / 4> pages, next;
+    if (part.begin + first >= part.end) return;
     pages.fetch(a, table, part.begin + first, part.end);
     for (int kb = part.begin + first; kb < part.end; kb += step, pages = next) {
         Row kr[KEYS], vr[KEYS];
@@ -811,19 +817,42 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(AttendArgs a) {
             sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// How a call is split, from what the host knows of it.
+// How a call is split, from what the host knows of it (the lengths are the
+// device's).
 struct Split {
-    int slots, workers, few, least, enough, cached;
+    int slots, workers, few, least, enough, cached;  // as in AttendArgs
     size_t ml_at, parts_at, bytes;  // offsets of the workspace's pieces; its size
 };
 
-constexpr int CUS = 256, WORKGROUPS_PER_CU = 8;
+constexpr int CUS = 256;
+
+// A split costs the join and the search for a part, about 4 us; a whole
+// sequence is bound by what one CU reads, about 70 GB/s. Measured, whole against
+// split, by the bytes of a sequence's keys and values of one head: 12
+// workgroups, 256 KB 7.8 and 7.9 us, 512 KB 12.5 and 8.1; 128 workgroups, 512
+// KB 15 and 20, 1 MB 33 and 29; 768 workgroups, 512 KB 75 and 84. The device
+// reads 70 times as fast as a CU, so with very many workgroups one longer
+// sequence still ends with the others.
 constexpr long long WHOLE_FEW = 256 << 10, WHOLE_MANY = 512 << 10;
 constexpr int MANY = 96;
-constexpr long long CACHES = 120000000;
+constexpr long long WHOLE_SHARE = 256;  // bytes a workgroup
 
-// Query heads of one kv head that a workgroup takes, and workgroups they need.
-constexpr int ROWS = 4;  // up to this many, fp32 queries go by attend_rows_kernel
+// Parts: up to 8 workgroups a CU in all, for balance (128 requests of 1 to 8192
+// tokens: 4 a CU 133 us, 8 129, 16 127; two of 131072: 172, 176, 186); parts
+// of at least 64 KB; parts of up to 256 KB while that leaves a workgroup a CU
+// (16 x 2000 tokens: parts of 64 KB 36 us, of 256 KB 31).
+constexpr int WORKGROUPS_PER_CU = 8;
+constexpr long long PART_LEAST = 64 << 10, PART_ENOUGH = 256 << 10;
+
+// Keys and values that pass the device's caches (256 MB, half of it what the
+// other tensors of a step leave) are read non-temporally: two contexts of
+// 131072 tokens 198 -> 177 us, 64 x 2000 tokens 105 -> 94; what fits is kept
+// (16 x 1000 tokens, 66 MB, read again and again: 14.9 us, non-temporally 20.6).
+constexpr double CACHES = 1.2e8;
+
+constexpr int ROWS = 4;  // query heads of a kv head up to which fp32 queries go by attend_rows_kernel
+
+// Workgroups that share a kv head's query heads.
 int tiles_of(const PagedCache &c, const PagedBatch &b) {
     const int group = b.heads / c.kv_heads;
     const int cols = b.type != BMB_F32 && group > 16 ? 32 : 16;
@@ -832,32 +861,31 @@ int tiles_of(const PagedCache &c, const PagedBatch &b) {
 
 Split split_of(const PagedCache &c, const PagedBatch &b) {
     Split s = {b.requests, 0, 0, 0, 0, 0, 0, 0, 0};
-    const long long rows = c.kv_heads * tiles_of(c, b);  // workgroups of one slot
+    const long long heads = (long long)c.kv_heads * tiles_of(c, b);  // workgroups of one slot
     const long long key_bytes = 2ll * c.head_size * element_size(c.type);
-    // (A whole sequence does not look at the others' lengths: half of the most they can be.)
-    s.cached = b.requests * (long long)b.max_len * key_bytes * c.kv_heads < 2 * CACHES;
-    const long long whole = b.requests * rows >= MANY ? WHOLE_MANY : WHOLE_FEW;
-    if (b.max_len * key_bytes > whole) {
-        long long workers = CUS * WORKGROUPS_PER_CU / rows;
-        workers = workers < 1 ? 1 : workers;
-        const long long units = (b.max_len + UNIT - 1) / UNIT;
-        const long long most = b.requests * units;
-        workers = workers < most ? workers : most;
-        s.workers = (int)workers;
-        s.cached = (int)(CACHES / (key_bytes * c.kv_heads * UNIT));
-        s.cached = s.cached < 1 ? 1 : s.cached;
-        s.few = CUS / rows < 1 ? 1 : (int)(CUS / rows);
-        const int least = (int)((64 << 10) / (key_bytes * UNIT));
-        s.least = least < 1 ? 1 : least;
-        s.enough = 4 * s.least;
-        const long long slots = b.requests + workers < most ? b.requests + workers : most;
-        s.slots = (int)slots;
-        const size_t o = (size_t)s.slots * b.heads * c.head_size * sizeof(float);
-        const size_t ml = (size_t)s.slots * b.heads * sizeof(float2);
-        s.ml_at = o;
-        s.parts_at = o + ml;
-        s.bytes = o + ml + (size_t)b.requests * sizeof(int2);
-    }
+    const long long all = b.requests * heads;
+    // Whole sequences do not look at each other's lengths: the batch is taken
+    // for half of the most it can be.
+    s.cached = 0.5 * b.requests * b.max_len * key_bytes * c.kv_heads < CACHES;
+    long long whole = all >= MANY ? WHOLE_MANY : WHOLE_FEW;
+    if (whole < all * WHOLE_SHARE) whole = all * WHOLE_SHARE;
+    if (b.max_len * key_bytes <= whole) return s;
+
+    const auto at_least_1 = [](long long x) { return x < 1 ? 1ll : x; };
+    const long long units = (b.max_len + UNIT - 1) / UNIT, most = b.requests * units;
+    long long workers = at_least_1(CUS * WORKGROUPS_PER_CU / heads);
+    workers = workers < most ? workers : most;
+    s.workers = (int)workers;
+    s.slots = (int)(b.requests + workers < most ? b.requests + workers : most);
+    s.few = (int)at_least_1(CUS / heads);
+    s.least = (int)at_least_1(PART_LEAST / (key_bytes * UNIT));
+    s.enough = (int)at_least_1(PART_ENOUGH / (key_bytes * UNIT));
+    const double cached = CACHES / ((double)key_bytes * c.kv_heads * UNIT);
+    s.cached = cached < 1.0 ? 1 : (int)cached;
+    const size_t rows = (size_t)s.slots * b.heads;
+    s.ml_at = rows * c.head_size * sizeof(float);
+    s.parts_at = s.ml_at + rows * sizeof(float2);
+    s.bytes = s.parts_at + (size_t)b.requests * sizeof(int2);
     return s;
 }
 
@@ -866,6 +894,7 @@ const char *batch_fault(const PagedCache *c, const PagedBatch *b) {
     if (b == nullptr) return "no batch";
     if (b->requests < 1 || b->max_len < 0 || b->heads < 1 || b->n_rows < 1)
         return "a size is below its least";
+    if (b->max_len > INT_MAX - 4096) return "max_len is more than 2^31 - 4097";
     if (b->heads % c->kv_heads != 0) return "heads is no multiple of kv_heads";
     if (b->type != BMB_F32 && b->type != BMB_F16 && b->type != BMB_BF16)
         return "unknown element type";
@@ -879,6 +908,8 @@ const char *batch_fault(const PagedCache *c, const PagedBatch *b) {
     const long long size = element_size(b->type);
     if (b->q_stride * size % 4 != 0 || b->out_stride * size % 4 != 0)
         return "rows are no multiples of 4 bytes";
+    if (b->n_rows > 1 && b->out_stride < (long long)b->heads * c->head_size)
+        return "rows of out overlap";
     return nullptr;
 }
 

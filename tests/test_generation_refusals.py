@@ -106,6 +106,8 @@ def test_nothing_to_append_is_no_launch():
                                     (dict(max_len=65), "table_stride"),
                                     (dict(table_stride=3), "table_stride"),
                                     (dict(requests=1 << 29), "too many"),
+                                    (dict(max_len=(1 << 31) - 4096, table_stride=1 << 27), "4097"),
+                                    (dict(out_stride=255), "overlap"),
                                     (dict(block_table=None), "null"), (dict(lens=None), "null")])
 def test_attention_refuses(capfd, kw, why):
     refused(capfd, why, bmb.paged_attention, cache(), batch(**kw), P, P, P)

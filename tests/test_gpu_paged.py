@@ -178,13 +178,25 @@ def test_attention_edges(gpu, type, cache, hs, heads, kv, page, layout):
 @pytest.mark.parametrize("hs", [32, 64, 128])
 @pytest.mark.parametrize("lens,heads,kv,page", [([4500], 12, 12, 16), ([257, 0, 1, 2500], 8, 2, 24),
                                                 ([3000, 2], 20, 1, 32), ([2600, 129], 3, 1, 48), ([2500, 700], 40, 1, 10),
-                                                ([300] * 70 + [0, 1, 5000], 2, 2, 16)])
+                                                ([300] * 70 + [0, 1, 5000], 2, 2, 16),
+                                                ([40] * 190 + [9000], 2, 2, 8)])
 def test_attention_split(gpu, type, cache, hs, lens, heads, kv, page):
     print("attention split", type, cache, hs, lens[:4], heads, kv, page, flush=True)
     p = Problem(lens, heads, kv, hs, type, cache, page, "head", seed=hs).device()
     assert p.workspace() > 0
     p.run()
     p.check()
+
+
+@pytest.mark.parametrize("type,cache", [("f32", "f32"), ("f16", "f16")])
+def test_attention_many_requests(gpu, type, cache):
+    """More workgroups than the device holds at once, every request whole."""
+    lens = [(7 * i) % 61 for i in range(1500)]
+    lens[1234] = 1300
+    d = Problem(lens, 4, 2, 64, type, cache, 16, seed=16).device()
+    assert bmb.paged_attention_workspace(d.cache, d.batch) == 0
+    d.run()
+    d.check()
 
 
 @pytest.mark.parametrize("type,cache", [("f32", "f32"), ("bf16", "bf16")])
@@ -264,6 +276,38 @@ def test_attention_longer_than_max_len(gpu):
     d.run()
     torch.cuda.synchronize()
     d.p.lens = [96, 96]
+    d.check()
+
+
+def test_attention_of_no_tokens(gpu):
+    """max_len 0: every request is empty, and its table is not looked at."""
+    d = Problem([3, 40], 2, 2, 64, "bf16", "bf16", 16, seed=7).device()
+    d.batch.max_len, d.batch.table_stride = 0, 0
+    d.run()
+    torch.cuda.synchronize()
+    d.p.lens = [0, 0]
+    d.check()
+
+
+@pytest.mark.parametrize("type,cache", TYPES)
+def test_attention_subnormal_values(gpu, type, cache):
+    """fp16 values below 2^-14 (and results, where the type holds them) keep
+    their digits."""
+    p = Problem([50, 300], 8, 1, 64, type, cache, 16, seed=14)
+    p.v = (p.v.float() * 2.0 ** -19).to(p.v.dtype)
+    p.k = torch.where(torch.rand(p.k.shape, generator=torch.Generator().manual_seed(1)) < 0.3,
+                      (p.k.float() * 2.0 ** -19).to(p.k.dtype), p.k)
+    d = p.device()
+    d.run()
+    d.check()
+
+
+def test_attention_broadcast_query(gpu):
+    """q_stride 0: one query for all requests."""
+    d = Problem([20, 33, 900], 4, 2, 64, "f32", "f32", 16, seed=15).device()
+    d.batch.q_stride = 0
+    d.p.q[1:] = d.p.q[0]
+    d.run()
     d.check()
 
 
