@@ -66,6 +66,9 @@ __device__ __forceinline__ void block_scan(uint32_t &x, uint32_t &y, uint32_t &t
     y = add_sat(by, y);
 }
 
+// Latency, not bytes: a decoding step of 64 requests takes 4.2 us, 512 requests
+// with 260 000 prompt tokens 6.4, and a launch that does nothing about 2.
+//
 // Every workgroup scans all requests (pages asked for, tokens granted, pages
 // given back) into LDS and fills its share of the tokens from there: a search
 // of the offsets finds a token's request. A new page's first token is new by
@@ -198,7 +201,10 @@ template <typename T>
 using Vec8 __attribute__((ext_vector_type(8))) = T;
 
 // One thread moves eight elements of a key and of the value beside it. The
-// rows come at any multiple of 4 bytes, the cache in multiples of 16.
+// rows come at any multiple of 4 bytes, the cache in multiples of 16. Bound by
+// HBM: 65536 tokens of 8 heads of 128 in bf16 (537 MB read and written) take 104
+// us, 5.2 TB/s, the rate of a copy; 32 tokens 2.0 us, a launch. (Non-temporal
+// stores gain 2% there and lose a third where fp32 goes to fp32.)
 template <typename TS, typename TC, int HS>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr int PIECES = HS / 8;
