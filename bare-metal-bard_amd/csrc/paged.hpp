@@ -78,6 +78,8 @@ inline const char *cache_fault(const PagedCache *c) {
                                     (unsigned long long)(c->token_stride * size) |
                                     (unsigned long long)(c->head_stride * size);
     if (bits % 16 != 0) return "the cache's buffers and strides are no multiples of 16 bytes";
+    if (c->token_stride >= (1ll << 26))  // lanes' offsets: 16 rows in 32 bits
+        return "token_stride of the cache is 2^26 elements or more";
     if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0)
         return "negative stride of the cache";
     return nullptr;

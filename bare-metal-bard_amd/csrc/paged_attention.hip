@@ -156,12 +156,14 @@ __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) {
 
 // A load of the cache. NT: not kept in the caches behind it (non-temporal), for
 // batches that do not fit them anyway.
+// A wave-uniform base and 32 bits of each lane's own: no address arithmetic
+// in the vector unit.
 template <bool NT, typename R>
-__device__ __forceinline__ R load(const char *p) {
+__device__ __forceinline__ R load(const char *p, uint32_t lane) {
     if constexpr (NT)
-        return __builtin_nontemporal_load((const R *)p);
+        return __builtin_nontemporal_load((const R *)(p + lane));
     else
-        return *(const R *)p;
+        return *(const R *)(p + lane);
 }
 
 // What a wave holds of the queries and of one step's keys and values, and the
@@ -194,13 +196,13 @@ struct Half {
         for (int s = 0; s < HS / 32; ++s) q.q[s] = (V8)(T)0.0f;
     }
     template <bool NT>
-    static __device__ __forceinline__ void load_k(Regs &x, int t, const char *row, int g) {
+    static __device__ __forceinline__ void load_k(Regs &x, int t, const char *p, uint32_t lane) {
         for (int s = 0; s < HS / 32; ++s)
-            x.k[t][s] = load<NT, V8>(row + (s * 32 + g * 8) * sizeof(T));
+            x.k[t][s] = load<NT, V8>(p + s * 64, lane);
     }
     template <bool NT>
-    static __device__ __forceinline__ void load_v(Regs &x, int i, const char *row, int c) {
-        x.v[i] = load<NT, Row>(row + c * DPL * sizeof(T));
+    static __device__ __forceinline__ void load_v(Regs &x, int i, const char *p, uint32_t lane) {
+        x.v[i] = load<NT, Row>(p, lane);
     }
     static __device__ __forceinline__ void zero_v(Regs &x, int i) { x.v[i] = (Row)0u; }
     static __device__ __forceinline__ f32x4 scores(const Regs &x, int t, const Query &q) {
@@ -261,13 +263,13 @@ struct Full {
         for (int s = 0; s < HS / 4; ++s) q.q[s] = 0.0f;
     }
     template <bool NT>
-    static __device__ __forceinline__ void load_k(Regs &x, int t, const char *row, int g) {
+    static __device__ __forceinline__ void load_k(Regs &x, int t, const char *p, uint32_t lane) {
         for (int s = 0; s < HS / (4 * EPL); ++s)
-            x.k[t][s] = load<NT, VE>(row + (s * 4 + g) * 16);
+            x.k[t][s] = load<NT, VE>(p + s * 64, lane);
     }
     template <bool NT>
-    static __device__ __forceinline__ void load_v(Regs &x, int i, const char *row, int c) {
-        x.v[i] = load<NT, vec<T, DPL>>(row + c * DPL * sizeof(T));
+    static __device__ __forceinline__ void load_v(Regs &x, int i, const char *p, uint32_t lane) {
+        x.v[i] = load<NT, vec<T, DPL>>(p, lane);
     }
     static __device__ __forceinline__ void zero_v(Regs &x, int i) {
         x.v[i] = (vec<T, DPL>)(T)0.0f;
@@ -334,38 +336,60 @@ struct Pages {
     }
 };
 
-// Loads the step of keys from kb on. Returns which of the lane's KV keys (4g +
-// r of each 16) count.
+// Which keys of a step count.
+template <bool ALIGNED, int TILES>
+struct Live {
+    bool whole;  // all of them, for every lane
+    int n[TILES];   // ALIGNED: the first n of each tile
+    uint32_t bits;  // otherwise: by this lane's keys
+    // Of this lane's 4 * TILES keys, of which the r-th of a tile is its key
+    // `first` + r * `step`.
+    __device__ __forceinline__ uint32_t mask(int first, int step) const {
+        if constexpr (!ALIGNED) return bits;
+        uint32_t m = 0;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) m |= (first + r * step < n[t] ? 1u : 0u) << (4 * t + r);
+        return m;
+    }
+};
+
+// Loads the step of keys from kb on. k and v: a row's start in the cache's first
+// page, for the wave.
 template <typename P, bool ALIGNED, bool NT>
-__device__ __forceinline__ unsigned load_step(typename P::Regs &x, const AttendArgs &a,
-                                              const Pages<ALIGNED, P::TILES> &pages,
-                                              const char *k, const char *v, int kb, int end, int g,
-                                              int c) {
-    unsigned live = 0;
-    uint32_t place = 0;
-    if constexpr (!ALIGNED) place = pages.place(a, kb, end);
+__device__ __forceinline__ Live<ALIGNED, P::TILES> load_step(typename P::Regs &x,
+                                                             const AttendArgs &a,
+                                                             const Pages<ALIGNED, P::TILES> &pages,
+                                                             const char *k, const char *v, int kb,
+                                                             int end, int g, int c) {
+    Live<ALIGNED, P::TILES> live = {true, {}, 0};
+    const uint32_t row = (uint32_t)a.token_stride * P::SIZE;
+    const uint32_t k_at = g * 16, v_at = c * P::DPL * P::SIZE;  // in a row
+    if constexpr (ALIGNED) {
 #pragma unroll
-    for (int t = 0; t < P::TILES; ++t) {
-        if constexpr (ALIGNED) {
-            int n;
-            const long long at = pages.tile(a, t, kb, end, P::SIZE, n);
-            const long long row = a.token_stride * P::SIZE;
-            P::template load_k<NT>(x, t, k + at + c * row, g);
+        for (int t = 0; t < P::TILES; ++t) {
+            const long long at = pages.tile(a, t, kb, end, P::SIZE, live.n[t]);
+            live.whole &= live.n[t] == 16;
+            P::template load_k<NT>(x, t, k + at, c * row + k_at);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                P::template load_v<NT>(x, 4 * t + r, v + at + (4 * g + r) * row, c);
-                live |= (4 * g + r < n ? 1u : 0u) << (4 * t + r);
-            }
-        } else {
+            for (int r = 0; r < 4; ++r)
+                P::template load_v<NT>(x, 4 * t + r, v + at + r * (size_t)row, 4 * g * row + v_at);
+        }
+    } else {
+        const uint32_t place = pages.place(a, kb, end);
+#pragma unroll
+        for (int t = 0; t < P::TILES; ++t) {
             const uint32_t at = __shfl(place, 16 * t + c);
-            P::template load_k<NT>(x, t, k + (at == NO_ROW ? 0ull : at * 16ull), g);
+            P::template load_k<NT>(x, t, k + (at == NO_ROW ? 0ull : at * 16ull), k_at);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t to = __shfl(place, 16 * t + 4 * g + r);
-                P::template load_v<NT>(x, 4 * t + r, v + (to == NO_ROW ? 0ull : to * 16ull), c);
-                live |= (to != NO_ROW ? 1u : 0u) << (4 * t + r);
+                P::template load_v<NT>(x, 4 * t + r, v + (to == NO_ROW ? 0ull : to * 16ull), v_at);
+                live.bits |= (to != NO_ROW ? 1u : 0u) << (4 * t + r);
             }
         }
+        live.whole = __builtin_amdgcn_ballot_w64(place == NO_ROW) == 0;
     }
     return live;
 }
@@ -430,14 +454,15 @@ __device__ __forceinline__ void attend_steps(f32x4 (&o)[QT][P::DPL], float (&m)[
     for (int kb = part.begin + first; kb < part.end; kb += step, pages = next) {
         typename P::Regs x;
         next.fetch(a, table, kb + step, part.end);
-        const unsigned live = load_step<P, ALIGNED, NT>(x, a, pages, k, v, kb, part.end, g, c);
-        const bool whole = __builtin_amdgcn_ballot_w64(live != (1u << KV) - 1) == 0;
+        const auto live = load_step<P, ALIGNED, NT>(x, a, pages, k, v, kb, part.end, g, c);
+        const bool whole = live.whole;
+        const uint32_t on = whole ? 0u : live.mask(4 * g, 1);
         if (!whole) {
             // What lies in an absent place may be NaN or infinite: the value
             // (and the score, below) is replaced, not multiplied by 0.
 #pragma unroll
             for (int i = 0; i < KV; ++i)
-                if (!(live >> i & 1)) P::zero_v(x, i);
+                if (!(on >> i & 1)) P::zero_v(x, i);
         }
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
@@ -450,7 +475,7 @@ __device__ __forceinline__ void attend_steps(f32x4 (&o)[QT][P::DPL], float (&m)[
             }
             if (!whole) {
 #pragma unroll
-                for (int i = 0; i < KV; ++i) p[i] = live >> i & 1 ? p[i] : -INFINITY;
+                for (int i = 0; i < KV; ++i) p[i] = on >> i & 1 ? p[i] : -INFINITY;
             }
             float top = p[0];
 #pragma unroll
@@ -608,13 +633,13 @@ __device__ __forceinline__ constexpr int row_at(int c, int j) {
     return DPL <= E ? c * DPL + j : (j / E) * (HS / 2) + c * E + j % E;
 }
 template <typename T, int HS, bool NT>
-__device__ __forceinline__ vec<T, HS / 16> load_row(const char *p) {
+__device__ __forceinline__ vec<T, HS / 16> load_row(const char *p, uint32_t lane) {
     constexpr int DPL = HS / 16, E = 16 / sizeof(T);
     if constexpr (DPL <= E) {
-        return load<NT, vec<T, DPL>>(p);
+        return load<NT, vec<T, DPL>>(p, lane);
     } else {
-        const vec<T, E> x = load<NT, vec<T, E>>(p);
-        const vec<T, E> y = load<NT, vec<T, E>>(p + HS / 2 * sizeof(T));
+        const vec<T, E> x = load<NT, vec<T, E>>(p, lane);
+        const vec<T, E> y = load<NT, vec<T, E>>(p + HS / 2 * sizeof(T), lane);
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 }
@@ -622,24 +647,23 @@ __device__ __forceinline__ vec<T, HS / 16> load_row(const char *p) {
 // A step's rows of K and V, and which of the lane's keys (kb + 4 i + g) count; as
 // load_step.
 template <typename T, int HS, int KEYS, bool ALIGNED, bool NT>
-__device__ __forceinline__ unsigned load_rows(vec<T, HS / 16> (&kr)[KEYS],
-                                              vec<T, HS / 16> (&vr)[KEYS], const AttendArgs &a,
-                                              const Pages<ALIGNED, KEYS / 4> &pages,
-                                              const char *k, const char *v, int kb, int end,
-                                              int g) {
-    unsigned live = 0;
+__device__ __forceinline__ Live<ALIGNED, KEYS / 4> load_rows(
+    vec<T, HS / 16> (&kr)[KEYS], vec<T, HS / 16> (&vr)[KEYS], const AttendArgs &a,
+    const Pages<ALIGNED, KEYS / 4> &pages, const char *k, const char *v, int kb, int end, int g,
+    int c) {
+    Live<ALIGNED, KEYS / 4> live = {true, {}, 0};
+    const uint32_t row = (uint32_t)a.token_stride * (uint32_t)sizeof(T);
+    const uint32_t in_row = row_at<T, HS>(c, 0) * sizeof(T);
     if constexpr (ALIGNED) {
 #pragma unroll
         for (int t = 0; t < KEYS / 4; ++t) {
-            int n;
-            const long long at = pages.tile(a, t, kb, end, sizeof(T), n);
-            const long long row = a.token_stride * (int)sizeof(T);
+            const long long at = pages.tile(a, t, kb, end, sizeof(T), live.n[t]);
+            live.whole &= live.n[t] == 16;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const long long to = at + (4 * r + g) * row;
-                kr[4 * t + r] = load_row<T, HS, NT>(k + to);
-                vr[4 * t + r] = load_row<T, HS, NT>(v + to);
-                live |= (4 * r + g < n ? 1u : 0u) << (4 * t + r);
+                const size_t to = at + 4 * r * (size_t)row;
+                kr[4 * t + r] = load_row<T, HS, NT>(k + to, g * row + in_row);
+                vr[4 * t + r] = load_row<T, HS, NT>(v + to, g * row + in_row);
             }
         }
     } else {
@@ -647,11 +671,12 @@ __device__ __forceinline__ unsigned load_rows(vec<T, HS / 16> (&kr)[KEYS],
 #pragma unroll
         for (int i = 0; i < KEYS; ++i) {
             const uint32_t at = __shfl(place, 4 * i + g);
-            const unsigned long long to = at == NO_ROW ? 0ull : at * 16ull;
-            kr[i] = load_row<T, HS, NT>(k + to);
-            vr[i] = load_row<T, HS, NT>(v + to);
-            live |= (at != NO_ROW ? 1u : 0u) << i;
+            const size_t to = at == NO_ROW ? 0 : at * (size_t)16;
+            kr[i] = load_row<T, HS, NT>(k + to, in_row);
+            vr[i] = load_row<T, HS, NT>(v + to, in_row);
+            live.bits |= (at != NO_ROW ? 1u : 0u) << i;
         }
+        live.whole = __builtin_amdgcn_ballot_w64(place == NO_ROW) == 0;
     }
     return live;
 }
@@ -670,14 +695,15 @@ __device__ __forceinline__ void rows_steps(float (&acc)[G][HS / 16], float (&m)[
     for (int kb = part.begin + first; kb < part.end; kb += step, pages = next) {
         Row kr[KEYS], vr[KEYS];
         next.fetch(a, table, kb + step, part.end);
-        const unsigned live =
-            load_rows<T, HS, KEYS, ALIGNED, NT>(kr, vr, a, pages, k, v, kb, part.end, g);
-        const bool whole = __builtin_amdgcn_ballot_w64(live != (1u << KEYS) - 1) == 0;
+        const auto live =
+            load_rows<T, HS, KEYS, ALIGNED, NT>(kr, vr, a, pages, k, v, kb, part.end, g, c);
+        const bool whole = live.whole;
+        const uint32_t on = whole ? 0u : live.mask(g, 4);
         if (!whole) {
             // (the value itself is replaced: 0 times an infinity is no 0)
 #pragma unroll
             for (int i = 0; i < KEYS; ++i)
-                if (!(live >> i & 1)) vr[i] = (Row)(T)0.0f;
+                if (!(on >> i & 1)) vr[i] = (Row)(T)0.0f;
         }
 #pragma unroll
         for (int h = 0; h < G; ++h) {
@@ -689,7 +715,7 @@ __device__ __forceinline__ void rows_steps(float (&acc)[G][HS / 16], float (&m)[
                 for (int j = 1; j < DPL; ++j) s[i] = fma_rn(q[h][j], (float)kr[i][j], s[i]);
             }
             float x = spread_sum<KEYS>(s, c);
-            if (!whole) x = live >> (c & (KEYS - 1)) & 1 ? x : -INFINITY;
+            if (!whole) x = on >> (c & (KEYS - 1)) & 1 ? x : -INFINITY;
             const float m1 = fmaxf(m[h], row_max<KEYS>(x));
             const float ref = m1 == -INFINITY ? 0.0f : m1;
             const float keep = __builtin_amdgcn_exp2f(m[h] - ref);
@@ -724,8 +750,8 @@ __global__ __launch_bounds__(WAVES *WAVE) void attend_rows_kernel(AttendArgs a) 
     const int cols = min(a.group - tile * G, G);
     const int head0 = kv_head * a.group + tile * G;
     const int *table = a.table + (size_t)part.r * a.table_stride;
-    const long long lane_at = kv_head * a.head_stride + row_at<T, HS>(c, 0);
-    const char *k = a.k + lane_at * (int)sizeof(T), *v = a.v + lane_at * (int)sizeof(T);
+    const char *k = a.k + kv_head * a.head_stride * (int)sizeof(T);
+    const char *v = a.v + kv_head * a.head_stride * (int)sizeof(T);
 
     float q[G][DPL], acc[G][DPL], m[G], l[G];
 #pragma unroll

@@ -67,7 +67,8 @@ BAD_CACHES = [(dict(k=None), "no cache"), (dict(v=None), "no cache"), (dict(type
               (dict(k=P + 8), "16 bytes"), (dict(v=P + 4), "16 bytes"),
               (dict(page_stride=2046), "16 bytes"), (dict(token_stride=130), "16 bytes"),
               (dict(head_stride=65), "16 bytes"), (dict(type=bmb.F16, token_stride=132), "16 bytes"),
-              (dict(page_stride=-2048), "negative")]
+              (dict(page_stride=-2048), "negative"),
+              (dict(token_stride=1 << 26), "token_stride")]
 
 
 @pytest.mark.parametrize("kw,why", BAD_CACHES)
