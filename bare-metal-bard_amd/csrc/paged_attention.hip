@@ -732,7 +732,11 @@ __device__ __forceinline__ void rows_steps(float (&acc)[G][HS / 16], float (&m)[
 template <typename T, int HS, int G, bool ALIGNED, int WAVES>
 __global__ __launch_bounds__(WAVES *WAVE) void attend_rows_kernel(AttendArgs a) {
     constexpr int DPL = HS / 16, BYTES = DPL * sizeof(T);
-    constexpr int KEYS = BYTES >= 32 ? 4 : BYTES == 16 ? 8 : 16;  // 32 registers each of K and V
+    // Loads of a step, by a row's bytes a lane. Smaller steps start sooner and
+    // leave registers for more waves, until the loads in flight are too few
+    // (64 ragged sequences of bf16 heads of 64: 16 loads 13.7 us, 8 12.5; one
+    // short one 3.8 and 3.1; heads of 32: 16 20.9, 8 21.8, 4 27.6).
+    constexpr int KEYS = BYTES == 4 ? 16 : BYTES == 8 || (BYTES == 16 && sizeof(T) == 4) ? 8 : 4;
     constexpr int STEP = 4 * KEYS;
     extern __shared__ float merge[];
     float(*part_ml)[2][G] = (float(*)[2][G])merge;

@@ -153,7 +153,7 @@ int paged_plan(const PagedPlan *plan, struct ihipStream_t *stream);
  * cache's type. A row is kv_heads * head_size elements of `type` (BMB_F32, or
  * the cache's own), row_stride elements after the one before (3C in fused QKV
  * rows); rows are multiples of 4 bytes apart. Slots outside the cache (-1) are
- * skipped; a slot given twice keeps either row's values. */
+ * skipped; of a slot given twice, each 8 elements are either row's. */
 int paged_append(const PagedCache *cache, const void *k, const void *v, int type,
                  long long row_stride, const int *slots, int tokens, struct ihipStream_t *stream);
 
@@ -192,7 +192,10 @@ size_t paged_attention_workspace(const PagedCache *cache, const PagedBatch *batc
  * request's tokens; lse[row, h] (n_rows * heads floats, or null) is the natural
  * log-sum-exp of the scaled scores. A request without tokens, or whose every
  * score is -inf, gives 0 and -inf. Tokens in pages outside the cache count as
- * absent, and what lies in a page behind the last token has no influence. */
+ * absent, and what lies in a page behind the last token has no influence.
+ * Products and sums are fp32; with 16-bit queries a probability enters its
+ * products as two 16-bit numbers (2^-16 of it, or less, is lost), so there an
+ * infinite v_j gives NaN in its element of the result. */
 int paged_attention(const PagedCache *cache, const PagedBatch *batch, void *out, float *lse,
                     const void *q, struct ihipStream_t *stream);
 
