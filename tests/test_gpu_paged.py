@@ -6,6 +6,7 @@ Bars: paged_plan's whole numbers are equal; paged_append's elements are the
 rounded inputs, bit for bit; paged_attention is within the rounding bound that
 paged_util.Problem.exact derives for its sizes and types."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -22,6 +23,22 @@ EDGES = [0, 1, 15, 16, 17, 31, 32, 33, 127, 128, 129, 255, 256]
 
 
 # ------------------------------------------------------------------- plan
+def test_plan_of_many_tokens(gpu):
+    """More tokens than the workgroups have threads, long prompts beside single
+    tokens; on a side stream."""
+    r = np.random.default_rng(5)
+    lens = r.integers(0, 3000, 40)
+    lens[::4] = 0
+    pool = Pool(lens, 32, width=pages_of(45000, 32), free=14000, seed=6)
+    side = torch.cuda.Stream()
+    for in_place in (False, True):
+        new = np.ones(40, np.int64)
+        new[::4] = r.integers(1, 40000, 10)
+        new[3] = -1
+        torch.cuda.synchronize()
+        pool.step(new, int(new[new > 0].sum()) + 5, in_place, side.cuda_stream)
+
+
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("R,page,prompt", [(1, 16, 1), (1, 1, 3), (3, 5, 40), (64, 16, 1),
                                            (65, 16, 300), (1024, 8, 7), (1500, 3, 5),
@@ -403,6 +420,63 @@ def test_attention_captured(gpu):
         d.check()
         other.run()
         other.check()
+
+
+def test_attention_two_graphs_at_once(gpu):
+    """Two captured calls with a workspace each, replayed at once on two
+    streams: the eager bits, every time."""
+    problems = [Problem([3000, 5, 1200], 8, 2, 64, "bf16", "bf16", 16, seed=17),
+                Problem([900] * 9 + [0], 4, 4, 64, "f32", "f32", 12, seed=18)]
+    ds, graphs, streams, bits = [p.device() for p in problems], [], [], []
+    for d in ds:
+        assert d.workspace() > 0
+        d.run()
+        d.check()
+        bits.append(d.out.cpu().view(torch.int16).numpy().copy())
+        side = torch.cuda.Stream()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            d.run(side.cuda_stream)
+        graphs.append(g)
+        streams.append(side)
+    for _ in range(4):
+        for d in ds:
+            d.out.fill_(768.0)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for d, b in zip(ds, bits):
+            assert np.array_equal(d.out.cpu().view(torch.int16).numpy(), b)
+
+
+def test_attention_from_host_threads(gpu):
+    """Four host threads with leased scratch on the null stream at once."""
+    ds = [Problem([1500 + 100 * i, 40], 8, 2, 64, "f16", "f16", 16, seed=20 + i).device()
+          for i in range(4)]
+    torch.cuda.synchronize()
+    barrier, errors = threading.Barrier(4), []
+
+    def work(d):
+        try:
+            barrier.wait()
+            for _ in range(10):
+                d.run()
+            torch.cuda.synchronize()
+            bmb.check("paged_attention")
+        except Exception as e:  # reported by the main thread
+            errors.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(d,)) for d in ds]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    assert not any(t.is_alive() for t in threads) and not errors, errors
+    for d in ds:
+        d.check()
 
 
 # --------------------------------------------------------------- together
