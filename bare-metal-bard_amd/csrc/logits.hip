@@ -89,14 +89,15 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
                 for (int e = 0; e < N; ++e) x[i][e] = in[id + e];
             }
             if (mask)  // (a piece may reach into the next word)
-                bits[i] = __builtin_amdgcn_alignbit(mask[(id + N - 1) >> 5], mask[id >> 5], id & 31);
+                bits[i] =
+                    __builtin_amdgcn_alignbit(mask[(id + N - 1) >> 5], mask[id >> 5], id & 31);
         }
     }
 
-    // LDS: id's word at id - first + N.
+    // LDS: id's word at id + word.
     const bool counts = r.tokens != nullptr;
-    uint32_t *seen = (uint32_t *)lds + N - first;
-    uint32_t *bias = seen + (counts ? WORDS : 0);
+    const int word = N - first;
+    uint32_t *seen = (uint32_t *)lds, *bias = seen + (counts ? WORDS : 0);
     int b0 = 0, b1 = 0;
     if (r.bias_offsets) {
         b0 = min(max(r.bias_offsets[row], 0), r.biases);
@@ -120,15 +121,15 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
             for (int j = 0; j < AHEAD; ++j) {
                 if (id[j] < lo || id[j] >= hi) continue;
                 if (base + j * THREADS < prompt)
-                    atomicOr(&seen[id[j]], IN_PROMPT);
+                    atomicOr(&seen[id[j] + word], IN_PROMPT);
                 else
-                    atomicAdd(&seen[id[j]], 1u);
+                    atomicAdd(&seen[id[j] + word], 1u);
             }
         }
     }
     for (int i = b0 + tid; i < b1; i += THREADS) {
         const int id = r.bias_ids[i];
-        if (id >= lo && id < hi) atomicMax(&bias[id], (uint32_t)(i - b0) + 1);
+        if (id >= lo && id < hi) atomicMax(&bias[id + word], (uint32_t)(i - b0) + 1);
     }
     __syncthreads();
 
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
         if (counts) {
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
-                const uint4 w = *(const uint4 *)(seen + id + e);
+                const uint4 w = *(const uint4 *)(seen + (id + word + e));
                 n[e] = w.x, n[e + 1] = w.y, n[e + 2] = w.z, n[e + 3] = w.w;
                 any |= w.x | w.y | w.z | w.w;
             }
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
         if (biased) {
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
-                const uint4 w = *(const uint4 *)(bias + id + e);
+                const uint4 w = *(const uint4 *)(bias + (id + word + e));
                 entry[e] = w.x, entry[e + 1] = w.y, entry[e + 2] = w.z, entry[e + 3] = w.w;
                 any |= w.x | w.y | w.z | w.w;
             }
@@ -178,8 +179,8 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
     const int edge = tid < first - lo ? lo + tid : last + tid - (first - lo);
     if (edge < hi) {
         const bool on = !mask || (mask[edge >> 5] >> (edge & 31) & 1);
-        out[edge] = on ? one(in[edge], counts ? seen[edge] : 0, biased ? bias[edge] : 0)
-                       : (T)-INFINITY;
+        const uint32_t n = counts ? seen[edge + word] : 0, entry = biased ? bias[edge + word] : 0;
+        out[edge] = on ? one(in[edge], n, entry) : (T)-INFINITY;
     }
 }
 
@@ -201,7 +202,8 @@ void launch_logits(LogitsArgs &a, hipStream_t stream) {
     const int chunk = chunk_of<T>(few ? 1 : MOST);
     a.chunks = (a.V + chunk - 1) / chunk;
     const size_t words = chunk + 2 * piece_of<T>();
-    const size_t lds = ((a.r.tokens ? words : 0) + (a.r.bias_offsets ? words : 0)) * sizeof(uint32_t);
+    const int tables = (a.r.tokens != nullptr) + (a.r.bias_offsets != nullptr);
+    const size_t lds = tables * words * sizeof(uint32_t);
     launch(few    ? logits_kernel<T, 1, false>
            : past ? logits_kernel<T, MOST, true>
                   : logits_kernel<T, MOST, false>,

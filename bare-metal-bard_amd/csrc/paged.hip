@@ -165,7 +165,8 @@ __global__ __launch_bounds__(THREADS) void plan_kernel(PlanArgs a) {
             const int r = gone[i], have = a.page.quot(held[r] + p.page_size - 1);
             const int *row = p.block_table + (size_t)r * p.max_pages;
             const uint32_t to = head + count + first[r];
-            for (int j = tid & 63; j < have; j += WAVE) p.free_pages[(to + (uint32_t)j) % pages] = row[j];
+            for (int j = tid & 63; j < have; j += WAVE)
+                p.free_pages[(to + (uint32_t)j) % pages] = row[j];
         }
     }
     if (a.finish && blockIdx.x == 0) {
@@ -299,7 +300,8 @@ int paged_append(const PagedCache *c, const void *k, const void *v, int type, lo
     if (tokens < 0) return refuse(me, "negative number of tokens");
     if (tokens == 0) return 0;
     if (k == nullptr || v == nullptr || slots == nullptr) return refuse(me, "a null pointer");
-    if ((long long)tokens * c->kv_heads > INT_MAX) return refuse(me, "too many tokens for one call");
+    if ((long long)tokens * c->kv_heads > INT_MAX)
+        return refuse(me, "too many tokens for one call");
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(row_stride * size)) % 4 != 0)
         return refuse(me, "rows are no multiples of 4 bytes");
     AppendArgs a = {(const char *)k, (const char *)v, (char *)c->k, (char *)c->v, slots, row_stride,

@@ -891,7 +891,10 @@ constexpr long long PART_LEAST = 64 << 10, PART_ENOUGH = 256 << 10;
 // (16 x 1000 tokens, 66 MB, read again and again: 14.9 us, non-temporally 20.6).
 constexpr double CACHES = 1.2e8;
 
-constexpr int ROWS = 4;  // query heads of a kv head up to which fp32 queries go by attend_rows_kernel
+// Query heads of a kv head up to which fp32 queries go by attend_rows_kernel (8 take
+// too many registers there; 4, on 16 x 8000 keys of 64 in bf16: 33 us, 42 by the
+// matrix kernel).
+constexpr int ROWS = 4;
 
 // Workgroups that share a kv head's query heads.
 int tiles_of(const PagedCache &c, const PagedBatch &b) {
@@ -1062,7 +1065,8 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
                     tiles_of(*c, *b), c->pages, b->table_stride, b->max_len, b->n_rows,
                     s.slots, s.workers, s.few, s.least, s.enough, s.cached, b->scale * LOG2E,
                     FastDiv::of(c->page_size),
-                    (uint32_t)(c->page_stride * size / 16), (uint32_t)(c->token_stride * size / 16)};
+                    (uint32_t)(c->page_stride * size / 16),
+                    (uint32_t)(c->token_stride * size / 16)};
     const int hs = c->head_size;
     if (b->type == BMB_F16)
         launch_attend<_Float16, _Float16>(hs, a, stream);

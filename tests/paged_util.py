@@ -129,8 +129,8 @@ def cache_struct(k, v, layout, page, kv, hs, cache):
 class DeviceProblem:
     def __init__(self, p):
         self.p = p
-        lay = (lambda x: x.permute(0, 2, 1, 3).contiguous()) if p.layout == "head" else (lambda x: x)
-        self.k, self.v = lay(p.k).cuda(), lay(p.v).cuda()
+        self.k, self.v = (x.permute(0, 2, 1, 3).contiguous().cuda() if p.layout == "head"
+                          else x.cuda() for x in (p.k, p.v))
         self.table, self.lens = p.table.cuda(), ints(p.lens)
         self.rows = None if p.rows is None else ints(p.rows)
         self.q = p.q.cuda()
@@ -175,7 +175,8 @@ class DeviceProblem:
             o, z, ob, zb = exact[row]
             got = out[row, :W].view(p.heads, p.hs)
             bad = ~((got - o).abs() <= ob)
-            assert not bad.any(), (row, bad.nonzero()[:4].tolist(), got[bad][:4], o[bad][:4], ob[bad][:4])
+            assert not bad.any(), (row, bad.nonzero()[:4].tolist(), got[bad][:4], o[bad][:4],
+                                   ob[bad][:4])
             same = (lse[row] == z) | ((lse[row] - z).abs() <= zb)
             assert same.all(), (row, lse[row], z, zb)
             worst = max(worst, float(((got - o).abs() / (ob + 1e-300)).max()))

@@ -66,7 +66,8 @@ BAD_CACHES = [(dict(k=None), "no cache"), (dict(v=None), "no cache"), (dict(type
               (dict(head_size=256), "head size"), (dict(pages=1 << 27), "2^31"),
               (dict(k=P + 8), "16 bytes"), (dict(v=P + 4), "16 bytes"),
               (dict(page_stride=2046), "16 bytes"), (dict(token_stride=130), "16 bytes"),
-              (dict(head_stride=65), "16 bytes"), (dict(type=bmb.F16, token_stride=132), "16 bytes"),
+              (dict(head_stride=65), "16 bytes"),
+              (dict(type=bmb.F16, token_stride=132), "16 bytes"),
               (dict(page_stride=-2048), "negative"),
               (dict(token_stride=1 << 26), "token_stride")]
 
@@ -82,7 +83,8 @@ def test_cache_is_refused(capfd, kw, why):
 @pytest.mark.parametrize("kw,why", [(dict(type=7), "type"), (dict(type=bmb.F16), "own type"),
                                     (dict(tokens=-1), "negative"), (dict(k=None), "null"),
                                     (dict(v=None), "null"), (dict(slots=None), "null"),
-                                    (dict(k=P + 2), "4 bytes"), (dict(tokens=(1 << 30)), "too many")])
+                                    (dict(k=P + 2), "4 bytes"),
+                                    (dict(tokens=(1 << 30)), "too many")])
 def test_append_refuses(capfd, kw, why):
     a = dict(k=P, v=P, type=bmb.F32, row_stride=128, slots=P, tokens=4)
     a.update(kw)
@@ -146,7 +148,8 @@ def rules(**kw):
     return bmb.LogitsRules(**f)
 
 
-@pytest.mark.parametrize("kw,why", [(dict(lens=None), "lens"), (dict(token_stride=-1), "token_stride"),
+@pytest.mark.parametrize("kw,why", [(dict(lens=None), "lens"),
+                                    (dict(token_stride=-1), "token_stride"),
                                     (dict(tokens=None), "penalties"),
                                     (dict(bias_ids=None), "bias"), (dict(bias_values=None), "bias"),
                                     (dict(biases=-1), "bias"), (dict(mask_stride=3), "V bits"),

@@ -49,7 +49,8 @@ class Case:
         self.bias = (r.standard_normal(max(n, 1)) * 5).astype(np.float32)
         self.words = (V + 31) // 32 + 1
         self.masks = 3
-        self.mask = r.integers(0, 1 << 32, (self.masks, self.words), dtype=np.uint64).astype(np.uint32)
+        self.mask = r.integers(0, 1 << 32, (self.masks, self.words),
+                               dtype=np.uint64).astype(np.uint32)
         self.mask[1] = 0                                   # nothing is allowed
         self.index = r.integers(-1, self.masks + 1, rows)
         if rows > 3:
@@ -149,7 +150,8 @@ class Case:
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,V,stride", [(1, 1, None), (5, 65, 128), (4, 4095, None), (3, 4096, 4096),
+@pytest.mark.parametrize("rows,V,stride", [(1, 1, None), (5, 65, 128), (4, 4095, None),
+                                           (3, 4096, 4096),
                                            (4, 4097, 4100), (6, 50257, None), (5, 50257, 50304),
                                            (3, 12289, 12291), (70, 33, 33),
                                            # results past 32 MB, and just below

@@ -146,8 +146,9 @@ def test_plan_captured(gpu):
 
 # ----------------------------------------------------------------- append
 @pytest.mark.parametrize("type,cache", TYPES)
-@pytest.mark.parametrize("tokens,kv,hs,page,layout", [(1, 12, 64, 16, "token"), (37, 1, 32, 5, "head"),
-                                                      (300, 3, 128, 24, "head"), (257, 7, 64, 1, "token")])
+@pytest.mark.parametrize("tokens,kv,hs,page,layout",
+                         [(1, 12, 64, 16, "token"), (37, 1, 32, 5, "head"),
+                          (300, 3, 128, 24, "head"), (257, 7, 64, 1, "token")])
 def test_append(gpu, type, cache, tokens, kv, hs, page, layout):
     g = torch.Generator().manual_seed(tokens)
     pages = pages_of(tokens, page) + 2
@@ -194,7 +195,8 @@ def test_attention_edges(gpu, type, cache, hs, heads, kv, page, layout):
 @pytest.mark.parametrize("type,cache", TYPES)
 @pytest.mark.parametrize("hs", [32, 64, 128])
 @pytest.mark.parametrize("lens,heads,kv,page", [([4500], 12, 12, 16), ([257, 0, 1, 2500], 8, 2, 24),
-                                                ([3000, 2], 20, 1, 32), ([2600, 129], 3, 1, 48), ([2500, 700], 40, 1, 10),
+                                                ([3000, 2], 20, 1, 32), ([2600, 129], 3, 1, 48),
+                                                ([2500, 700], 40, 1, 10),
                                                 ([300] * 70 + [0, 1, 5000], 2, 2, 16),
                                                 ([40] * 190 + [9000], 2, 2, 8)])
 def test_attention_split(gpu, type, cache, hs, lens, heads, kv, page):
