@@ -891,8 +891,8 @@ constexpr long long PART_LEAST = 64 << 10, PART_ENOUGH = 256 << 10;
 // (16 x 1000 tokens, 66 MB, read again and again: 14.9 us, non-temporally 20.6).
 constexpr double CACHES = 1.2e8;
 
-// Query heads of a kv head up to which fp32 queries go by attend_rows_kernel (8 take
-// too many registers there; 4, on 16 x 8000 keys of 64 in bf16: 33 us, 42 by the
+// Query heads of a kv head up to which fp32 queries go by attend_rows_kernel, whose
+// registers grow with them (4, on 16 x 8000 keys of 64 in bf16: 33 us, 42 by the
 // matrix kernel).
 constexpr int ROWS = 4;
 
