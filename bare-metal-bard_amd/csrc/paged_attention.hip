@@ -49,7 +49,7 @@ struct AttendArgs {
     const int *table, *lens, *rows;
     float *part_o;     // (slots, heads, HS)
     float2 *part_ml;   // (slots, heads): running maximum (log2 units) and sum
-    int2 *parts;       // (requests): first slot, number of parts
+    int4 *parts;       // (requests): whole parts' first slot and number, the rest's slot or -1
     long long page_stride, token_stride, head_stride, q_stride, out_stride;
     int requests, heads, kv_heads, group, tiles, pages, table_stride, max_len, n_rows;
     int slots;          // parts that the launch has room for
@@ -64,7 +64,7 @@ struct AttendArgs {
 
 // The part of a request that a slot stands for; n: how many the request has (0: none here).
 struct Part {
-    int r, i, n, begin, end, row;
+    int r, i, n, whole, begin, end, row;  // (whole: those of full length, which come first)
     bool nt;  // the step's batch passes the caches
 };
 
@@ -77,13 +77,27 @@ __device__ __forceinline__ int len_of(const AttendArgs &a, int r) {
     return min(max(a.lens[r], 0), a.max_len);
 }
 
-// All parts are of one length, ceil(total / workers) units, so that their work
-// is alike whatever the lengths; the last part of each request is shorter.
-// (Sum of ceil(len / part) <= requests + workers: the slots.) Every wave finds
-// its slot's request by itself, 64 requests at a time.
+// The request, among 64 from `base` on, that the slot's count falls to: each has n
+// of them, `before` came earlier. Its lane, or -1; `before` moves on.
+__device__ __forceinline__ int find_lane(uint32_t n, uint32_t slot, uint32_t &before,
+                                         uint32_t &first) {
+    const uint32_t upto = before + wave_scan(n);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > slot);
+    before = __builtin_amdgcn_readlane(upto, 63);
+    if (past == 0) return -1;
+    const int l = __builtin_ctzll(past);
+    first = __builtin_amdgcn_readlane(upto - n, l);
+    return l;
+}
+
+// All parts are of one length, `size` units, whatever the sequences' lengths, but
+// for what is left of each sequence; those rests (and the sequences shorter than a
+// part) come behind the whole parts, so that the device ends on the short ones.
+// (Sum of ceil(len / part) <= requests + workers: the slots.) Every wave finds its
+// slot's request by itself, 64 requests at a time.
 __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
-    Part p = {slot, 0, 0, 0, 0, -1, a.cached == 0 && a.tiles == 1};
+    Part p = {slot, 0, 0, 0, 0, 0, -1, a.cached == 0 && a.tiles == 1};
     if (a.workers == 0) {
         p.row = row_of(a, slot);
         p.n = p.row >= 0;
@@ -101,23 +115,23 @@ __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
     uint32_t size = (total + a.workers - 1) / a.workers;
     size = max(size, min((total + a.few - 1) / a.few, (uint32_t)a.enough));
     size = max(size, (uint32_t)a.least);
-    uint32_t before = 0;
-    for (int base = 0; base < a.requests; base += WAVE) {
-        const int r = base + lane;
-        int len = 0, row = -1;
-        uint32_t n = 0;
-        if (r < a.requests) {
-            row = row_of(a, r);
-            len = len_of(a, r);
-            if (row >= 0) n = max(((len + UNIT - 1) / UNIT + size - 1) / size, 1u);
-        }
-        const uint32_t upto = before + wave_scan(n);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > (uint32_t)slot);
-        if (past) {
-            const int l = __builtin_ctzll(past);
+    uint32_t before = 0, first = 0;
+    for (int rests = 0; rests < 2; ++rests) {
+        for (int base = 0; base < a.requests; base += WAVE) {
+            const int r = base + lane;
+            int len = 0, row = -1;
+            if (r < a.requests) {
+                row = row_of(a, r);
+                len = len_of(a, r);
+            }
+            const uint32_t units = (len + UNIT - 1) / UNIT, whole = units / size;
+            const uint32_t rest = whole * size < units || units == 0;
+            const int l = find_lane(row < 0 ? 0 : rests ? rest : whole, slot, before, first);
+            if (l < 0) continue;
             p.r = base + l;
-            p.n = __builtin_amdgcn_readlane(n, l);
-            p.i = slot - (int)(__builtin_amdgcn_readlane(upto, l) - p.n);
+            p.whole = __builtin_amdgcn_readlane(whole, l);
+            p.n = p.whole + __builtin_amdgcn_readlane(rest, l);
+            p.i = rests ? p.whole : slot - (int)first;
             p.row = __builtin_amdgcn_readlane(row, l);
             p.end = __builtin_amdgcn_readlane(len, l);
             const long long keys = (long long)size * UNIT;
@@ -125,7 +139,6 @@ __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
             p.end = (int)min((long long)p.end, p.begin + keys);
             return p;
         }
-        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return p;
 }
@@ -435,8 +448,15 @@ __device__ __forceinline__ void merge_waves(const AttendArgs &a, const Part &par
             if (d == 0) a.part_ml[at] = make_float2(top, sum);
         }
     }
-    if (a.workers && threadIdx.x == 0 && part.i == 0 && head0 == 0)
-        a.parts[part.r] = make_int2(slot, part.n);
+    if (a.workers && threadIdx.x == 0 && head0 == 0) {
+        int4 &parts = a.parts[part.r];
+        if (part.i == part.whole) parts.z = slot;
+        if (part.i == 0) {
+            parts.x = slot;
+            parts.y = part.whole;
+            if (part.n == part.whole) parts.z = -1;
+        }
+    }
 }
 
 // A wave's share of a part: steps of keys from `first` on, `step` apart, for QT
@@ -816,12 +836,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(AttendArgs a) {
     __shared__ float sum_s[SHARES], top_s[SHARES];
     const int r = blockIdx.x / a.heads, head = blockIdx.x % a.heads, tid = threadIdx.x;
     const int row = row_of(a, r), len = len_of(a, r);
-    const int2 parts = a.parts[r];
-    if ((row < 0) | (len <= UNIT) | (parts.y < 2)) return;  // (one wait for the three loads)
+    const int4 parts = a.parts[r];
+    const int n = parts.y + (parts.z >= 0);
+    if ((row < 0) | (len <= UNIT) | (n < 2)) return;  // (one wait for the three loads)
     const int d = tid % LANES, share = tid / LANES;
-    const long long at = (long long)parts.x * a.heads + head;
-    const float2 *ml = a.part_ml + at;
-    const float *po = a.part_o + at * HS + 4 * d;
     float top = -INFINITY, sum = 0.0f;
     float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const auto add = [&](float m, float l, float4 y) {
@@ -835,10 +853,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(AttendArgs a) {
         acc.w = acc.w * f + y.w * e;
     };
 #pragma unroll 4
-    for (int i = share; i < parts.y; i += SHARES) {
-        const long long s = (long long)i * a.heads;
-        const float2 x = ml[s];
-        add(x.x, x.y, ld4(po + s * HS));
+    for (int i = share; i < n; i += SHARES) {
+        const int slot = i < parts.y ? parts.x + i : parts.z;
+        const long long at = (long long)slot * a.heads + head;
+        const float2 x = a.part_ml[at];
+        add(x.x, x.y, ld4(a.part_o + at * HS + 4 * d));
     }
     acc_s[share][d] = acc;
     if (d == 0) {
@@ -928,8 +947,8 @@ Split split_of(const PagedCache &c, const PagedBatch &b) {
     s.cached = cached < 1.0 ? 1 : (int)cached;
     const size_t rows = (size_t)s.slots * b.heads;
     s.ml_at = rows * c.head_size * sizeof(float);
-    s.parts_at = s.ml_at + rows * sizeof(float2);
-    s.bytes = s.parts_at + (size_t)b.requests * sizeof(int2);
+    s.parts_at = (s.ml_at + rows * sizeof(float2) + 15) / 16 * 16;
+    s.bytes = s.parts_at + (size_t)b.requests * sizeof(int4);
     return s;
 }
 
@@ -1060,7 +1079,7 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
     const int group = b->heads / c->kv_heads;
     AttendArgs a = {(const char *)q, (const char *)c->k, (const char *)c->v, (char *)out, lse,
                     b->block_table, b->lens, b->rows, (float *)work, (float2 *)(work + s.ml_at),
-                    (int2 *)(work + s.parts_at), c->page_stride, c->token_stride, c->head_stride,
+                    (int4 *)(work + s.parts_at), c->page_stride, c->token_stride, c->head_stride,
                     b->q_stride, b->out_stride, b->requests, b->heads, c->kv_heads, group,
                     tiles_of(*c, *b), c->pages, b->table_stride, b->max_len, b->n_rows,
                     s.slots, s.workers, s.few, s.least, s.enough, s.cached, b->scale * LOG2E,
