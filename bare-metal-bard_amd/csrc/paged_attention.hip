@@ -77,24 +77,32 @@ __device__ __forceinline__ int len_of(const AttendArgs &a, int r) {
     return min(max(a.lens[r], 0), a.max_len);
 }
 
-// The request, among 64 from `base` on, that the slot's count falls to: each has n
-// of them, `before` came earlier. Its lane, or -1; `before` moves on.
-__device__ __forceinline__ int find_lane(uint32_t n, uint32_t slot, uint32_t &before,
-                                         uint32_t &first) {
-    const uint32_t upto = before + wave_scan(n);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > slot);
-    before = __builtin_amdgcn_readlane(upto, 63);
-    if (past == 0) return -1;
-    const int l = __builtin_ctzll(past);
-    first = __builtin_amdgcn_readlane(upto - n, l);
-    return l;
+// A request's tokens, in units, and how they come apart: whole parts of `size` units
+// and a rest (an empty sequence is one empty rest).
+struct Asks {
+    int row, len;
+    uint32_t units, whole, rest;
+};
+__device__ __forceinline__ Asks asks_of(const AttendArgs &a, int r, uint32_t size) {
+    Asks x = {-1, 0, 0, 0, 0};
+    if (r < a.requests) {
+        x.row = row_of(a, r);
+        x.len = len_of(a, r);
+    }
+    if (x.row < 0) return x;
+    x.units = (x.len + UNIT - 1) / UNIT;
+    x.whole = x.units / size;
+    x.rest = x.whole * size < x.units || x.units == 0;
+    return x;
 }
 
 // All parts are of one length, `size` units, whatever the sequences' lengths, but
 // for what is left of each sequence; those rests (and the sequences shorter than a
 // part) come behind the whole parts, so that the device ends on the short ones.
 // (Sum of ceil(len / part) <= requests + workers: the slots.) Every wave finds its
-// slot's request by itself, 64 requests at a time.
+// slot's request by itself: each lane counts a share of the requests, which takes
+// three scans however many they are, then the wave looks into the share that holds
+// the slot.
 __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
     Part p = {slot, 0, 0, 0, 0, 0, -1, a.cached == 0 && a.tiles == 1};
@@ -104,42 +112,53 @@ __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
         p.end = len_of(a, slot);
         return p;
     }
-    uint32_t total = 0;
-    for (int base = 0; base < a.requests; base += WAVE) {
-        const int r = base + lane;
-        uint32_t units = 0;
-        if (r < a.requests && row_of(a, r) >= 0) units = (len_of(a, r) + UNIT - 1) / UNIT;
-        total += __builtin_amdgcn_readlane(wave_scan(units), 63);
-    }
+    const int share = (a.requests + WAVE - 1) / WAVE;
+    uint32_t units = 0;
+    for (int i = 0; i < share; ++i) units += asks_of(a, lane * share + i, 1).units;
+    const uint32_t total = __builtin_amdgcn_readlane(wave_scan(units), 63);
     p.nt = total >= (uint32_t)a.cached && a.tiles == 1;  // (several tiles read the same rows)
     uint32_t size = (total + a.workers - 1) / a.workers;
     size = max(size, min((total + a.few - 1) / a.few, (uint32_t)a.enough));
     size = max(size, (uint32_t)a.least);
-    uint32_t before = 0, first = 0;
-    for (int rests = 0; rests < 2; ++rests) {
-        for (int base = 0; base < a.requests; base += WAVE) {
-            const int r = base + lane;
-            int len = 0, row = -1;
-            if (r < a.requests) {
-                row = row_of(a, r);
-                len = len_of(a, r);
+
+    uint32_t whole = 0, rest = 0;
+    Asks x;
+    for (int i = 0; i < share; ++i) {
+        x = asks_of(a, lane * share + i, size);
+        whole += x.whole;
+        rest += x.rest;
+    }
+    const uint32_t whole_upto = wave_scan(whole), rest_upto = wave_scan(rest);
+    const uint32_t all_whole = __builtin_amdgcn_readlane(whole_upto, 63);
+    const bool rests = (uint32_t)slot >= all_whole;
+    uint32_t left = rests ? slot - all_whole : slot;  // slots before this one, from here on
+    const uint32_t upto = rests ? rest_upto : whole_upto;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > left);
+    if (past == 0) return p;
+    int l = __builtin_ctzll(past);
+    left -= __builtin_amdgcn_readlane(upto - (rests ? rest : whole), l);
+    p.r = l * share;
+    if (share > 1) {
+        for (int base = 0;; base += WAVE) {  // (ends: the share holds the slot)
+            x = asks_of(a, base + lane < share ? p.r + base + lane : a.requests, size);
+            const uint32_t n = rests ? x.rest : x.whole, sum = wave_scan(n);
+            const uint64_t here = __builtin_amdgcn_ballot_w64(sum > left);
+            l = here ? __builtin_ctzll(here) : 63;
+            left -= __builtin_amdgcn_readlane(here ? sum - n : sum, l);
+            if (here || base + WAVE >= share) {
+                p.r += base + l;
+                break;
             }
-            const uint32_t units = (len + UNIT - 1) / UNIT, whole = units / size;
-            const uint32_t rest = whole * size < units || units == 0;
-            const int l = find_lane(row < 0 ? 0 : rests ? rest : whole, slot, before, first);
-            if (l < 0) continue;
-            p.r = base + l;
-            p.whole = __builtin_amdgcn_readlane(whole, l);
-            p.n = p.whole + __builtin_amdgcn_readlane(rest, l);
-            p.i = rests ? p.whole : slot - (int)first;
-            p.row = __builtin_amdgcn_readlane(row, l);
-            p.end = __builtin_amdgcn_readlane(len, l);
-            const long long keys = (long long)size * UNIT;
-            p.begin = (int)(p.i * keys);
-            p.end = (int)min((long long)p.end, p.begin + keys);
-            return p;
         }
     }
+    p.whole = __builtin_amdgcn_readlane(x.whole, l);
+    p.n = p.whole + __builtin_amdgcn_readlane(x.rest, l);
+    p.i = rests ? p.whole : left;
+    p.row = __builtin_amdgcn_readlane(x.row, l);
+    p.end = __builtin_amdgcn_readlane(x.len, l);
+    const long long keys = (long long)size * UNIT;
+    p.begin = (int)(p.i * keys);
+    p.end = (int)min((long long)p.end, p.begin + keys);
     return p;
 }
 
