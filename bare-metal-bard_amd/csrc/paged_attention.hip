@@ -7,7 +7,7 @@
 // so the bound is the cache's bytes.
 //
 // Measured: two contexts of 131072 tokens, 8 kv heads of 128 in bf16 (1.07 GB)
-// 176 us back to back in a graph, 6.1 TB/s; an fp32 cache (460 MB) 5.9 TB/s; a
+// 175 us back to back in a graph, 6.1 TB/s; an fp32 cache (460 MB) 6.1 TB/s; a
 // plain copy moves 5.1 TB/s here. A single sequence of 1000 tokens takes 7.6 us
 // in two launches: latency.
 //
@@ -102,7 +102,8 @@ __device__ __forceinline__ Asks asks_of(const AttendArgs &a, int r, uint32_t siz
 // (Sum of ceil(len / part) <= requests + workers: the slots.) Every wave finds its
 // slot's request by itself: each lane counts a share of the requests, which takes
 // three scans however many they are, then the wave looks into the share that holds
-// the slot.
+// the slot. (Rests among the whole parts: 16 sequences of 3000-4000 tokens 79.5 us,
+// behind them 76.1; 256 requests, 64 to a scan: 81.3 us, in shares 78.2.)
 __device__ __forceinline__ Part find_part(const AttendArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
     Part p = {slot, 0, 0, 0, 0, 0, -1, a.cached == 0 && a.tiles == 1};
@@ -917,7 +918,7 @@ constexpr int MANY = 96;
 constexpr long long WHOLE_SHARE = 256;  // bytes a workgroup
 
 // Parts: up to 8 workgroups a CU in all, for balance (128 requests of 1 to 8192
-// tokens: 4 a CU 133 us, 8 129, 16 127; two of 131072: 172, 176, 186); parts
+// tokens: 4 a CU 135 us, 8 123, 16 124; two of 131072: 172, 175, 183); parts
 // of at least 64 KB; parts of up to 256 KB while that leaves a workgroup a CU
 // (16 x 2000 tokens: parts of 64 KB 36 us, of 256 KB 31).
 constexpr int WORKGROUPS_PER_CU = 8;
