@@ -204,14 +204,17 @@ __device__ __forceinline__ R load(const char *p, uint32_t lane) {
 //
 // 16-bit cache and queries: 16-bit products (exact in fp32), 32 keys a step.
 // The probabilities go in as a 16-bit rounding and the 16-bit rounding of what
-// it left (2^-16 of a probability in bf16, 2^-22 in fp16): a single bf16 (2^-9)
-// would add as much error as the result's own rounding, and the second product
-// costs nothing beside the loads.
+// it left: a single bf16 would add as much error as the result's own rounding,
+// and the second product costs nothing beside the loads. What the two lose is
+// at most 2^-17 of a probability in bf16 and 2^-23 in fp16, or there, if that is
+// more, 2^-40 of the largest: fp16 holds nothing below 2^-24, so probabilities
+// (at most 1) go in times 2^15, which the sums carry until the wave's end.
 template <typename T, int HS>
 struct Half {
     using Q = T;
     static constexpr int SIZE = sizeof(T);
     static constexpr int TILES = 2, KV = 4 * TILES, DPL = HS / 16;
+    static constexpr float P_SCALE = __is_same(T, _Float16) ? 0x1p15f : 1.0f;
     using V8 = vec<T, 8>;
     using Row = vec<uint32_t, DPL / 2>;
     struct Query {
@@ -249,8 +252,9 @@ struct Half {
         V8 hi, lo;
 #pragma unroll
         for (int i = 0; i < KV; ++i) {
-            hi[i] = (T)p[i];
-            lo[i] = (T)(p[i] - (float)hi[i]);
+            const float x = p[i] * P_SCALE;
+            hi[i] = (T)x;
+            lo[i] = (T)(x - (float)hi[i]);
         }
 #pragma unroll
         for (int j = 0; j < DPL; ++j) {
@@ -275,6 +279,7 @@ struct Full {
     static constexpr int SIZE = sizeof(T);
     // (32 keys of 16-bit heads of 128 take too many registers: 64 -> 82 us.)
     static constexpr int TILES = sizeof(T) == 2 && HS <= 64 ? 2 : 1, KV = 4 * TILES, DPL = HS / 16;
+    static constexpr float P_SCALE = 1.0f;
     static constexpr int EPL = 16 / sizeof(T);  // elements of a 16-byte load
     using VE = vec<T, EPL>;
     struct Query {
@@ -600,7 +605,8 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int j = 0; j < DPL; ++j)
-                    part_o[(wave * cols + col) * HS + (4 * g + r) * DPL + j] = o[u][j][r];
+                    part_o[(wave * cols + col) * HS + (4 * g + r) * DPL + j] =
+                        o[u][j][r] * (1.0f / P::P_SCALE);
         }
     }
     merge_waves<TQ, HS, WAVES, COLS>(a, part, slot, head0, cols);

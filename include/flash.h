@@ -194,8 +194,10 @@ size_t paged_attention_workspace(const PagedCache *cache, const PagedBatch *batc
  * score is -inf, gives 0 and -inf. Tokens in pages outside the cache count as
  * absent, and what lies in a page behind the last token has no influence.
  * Products and sums are fp32; with 16-bit queries a probability enters its
- * products as two 16-bit numbers (2^-16 of it, or less, is lost), so there an
- * infinite v_j gives NaN in its element of the result. */
+ * products as two 16-bit numbers, so there an infinite v_j gives NaN in its
+ * element of the result. What they lose is at most 2^-17 of a probability in
+ * bf16, and in fp16 2^-23 of it or, if that is more, 2^-40 of the request's
+ * largest. */
 int paged_attention(const PagedCache *cache, const PagedBatch *batch, void *out, float *lse,
                     const void *q, struct ihipStream_t *stream);
 

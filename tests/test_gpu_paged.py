@@ -14,7 +14,7 @@ import torch
 
 import bmb
 import oracle as O
-from paged_util import DTYPES, Pool, Problem, cache_struct, ints, pages_of, plan_exact
+from paged_util import DTYPES, U32, Pool, Problem, cache_struct, ints, pages_of, plan_exact
 
 pytestmark = pytest.mark.gpu
 
@@ -238,6 +238,50 @@ def test_attention_sharp_and_negative_scale(gpu, type, cache):
                     seed=4).device()
         d.run()
         d.check()
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,page", [(2, 16), (5, 10), (40, 16)])
+@pytest.mark.parametrize("gap", [8, 14, 18, 20])
+def test_attention_weak_keys_beside_a_strong_one(gpu, type, heads, page, gap):
+    """One key `gap` nats above all others, its value 0, theirs large: the result
+    is what the weak keys bring, to its last bits.
+
+    The bound is Problem.exact's, but for what the two 16-bit numbers of a
+    probability lose: at most 2^-17 (bf16) or 2^-23 (fp16) of it, and in fp16 up
+    to 2^-40 of the largest, once for each key."""
+    lens = [2, 40, 700, 3000, 129]
+    strong = [0, 39, 350, 2999, 17]
+    p = Problem(lens, heads, 1, 64, type, type, page, seed=gap)
+    p.q.zero_()
+    p.q[:, :heads * 64:64] = 1.0  # the score is scale times the key's first element
+    p.scale = gap / 16.0
+    g = torch.Generator().manual_seed(gap)
+    for r, n in enumerate(lens):
+        t = torch.arange(n)
+        at = (p.table[r].long()[t // page], t % page)
+        p.k[at] = 0.0
+        p.v[at] = (30000.0 + 30000.0 * torch.rand(n, 1, 64, generator=g)).to(p.v.dtype)
+        one = (int(p.table[r, strong[r] // page]), strong[r] % page)
+        p.k[one] = 16.0
+        p.v[one] = 0.0
+    d = p.device()
+    d.run()
+    torch.cuda.synchronize()
+    bmb.check("paged_attention")
+    half_step, lost = torch.finfo(DTYPES[type]).eps / 2, 2.0 ** (-17 if type == "bf16" else -23)
+    for r, (want, lse, _, lse_bound) in p.exact().items():
+        n = lens[r]
+        ds = 4 * (math.sqrt(64) + 1) * U32 * gap + 4 * U32 * gap
+        eps = 2 * ds + (4 * math.sqrt(n) + 16) * U32 + lost
+        # (all values are at least 0: the sum of their magnitudes is the result)
+        bound = (eps + half_step) * want
+        if type == "f16":
+            bound = bound + 2.0 ** -40 * 60000 * n + 2.0 ** -25
+        got = d.out[r, :heads * 64].cpu().double().view(heads, 64)
+        worst = ((got - want).abs() / bound).max().item()
+        assert worst <= 1.0, (r, n, worst, got[0, :4], want[0, :4])
+        assert ((d.lse[r].cpu().double() - lse).abs() <= lse_bound).all()
 
 
 @pytest.mark.parametrize("type,cache", TYPES)
