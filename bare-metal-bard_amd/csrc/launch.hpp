@@ -52,4 +52,14 @@ inline void launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
     note_launch_status(hipGetLastError());
 }
 
+// `blocks` workgroups of `threads` lanes in as many launches as that takes: a
+// dispatch holds fewer than 2^32 lanes. go(first, n): workgroups [first, first
+// + n). (Each launch starts on the first XCD: n is a multiple of 8, or the rest.)
+template <class F>
+inline void in_launches(long long blocks, int threads, F &&go) {
+    const long long most = ((1ll << 32) - 1) / threads / 8 * 8;
+    for (long long first = 0; first < blocks; first += most)
+        go(first, (unsigned)(blocks - first < most ? blocks - first : most));
+}
+
 }  // namespace bmb

@@ -26,6 +26,7 @@ struct LogitsArgs {
     const char *logits;
     long long stride;
     int rows, V, chunks;
+    int first;  // the launch's first workgroup of the call's
 };
 
 // Each operation rounds once, as written (no contraction).
@@ -56,7 +57,8 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
     typedef T Piece __attribute__((ext_vector_type(N)));
     extern __shared__ uint4 lds[];
     const LogitsRules &r = a.r;
-    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
+    const uint32_t block = a.first + blockIdx.x;
+    const int row = block / a.chunks, chunk = block % a.chunks, tid = threadIdx.x;
     T *out = (T *)a.out + row * a.stride;
     const T *in = (const T *)a.logits + row * a.stride;
     // Pieces start where the output row is a multiple of 16 bytes: `skew` ids
@@ -204,10 +206,13 @@ void launch_logits(LogitsArgs &a, hipStream_t stream) {
     const size_t words = chunk + 2 * piece_of<T>();
     const int tables = (a.r.tokens != nullptr) + (a.r.bias_offsets != nullptr);
     const size_t lds = tables * words * sizeof(uint32_t);
-    launch(few    ? logits_kernel<T, 1, false>
-           : past ? logits_kernel<T, MOST, true>
-                  : logits_kernel<T, MOST, false>,
-           dim3((unsigned)(a.chunks * a.rows)), dim3(THREADS), lds, stream, a);
+    const auto kernel = few    ? logits_kernel<T, 1, false>
+                        : past ? logits_kernel<T, MOST, true>
+                               : logits_kernel<T, MOST, false>;
+    in_launches((long long)a.chunks * a.rows, THREADS, [&](long long first, unsigned n) {
+        a.first = (int)first;
+        launch(kernel, dim3(n), dim3(THREADS), lds, stream, a);
+    });
 }
 
 int refuse(const char *why) {
@@ -245,7 +250,7 @@ extern "C" int logits_process(void *out, const void *logits, int type, int rows,
     if (r->mask && !r->mask_index && r->masks < rows) return refuse("fewer masks than rows");
     if ((V + 1023ll) / 1024 * rows > INT_MAX || V > INT_MAX - 16384)
         return refuse("too many logits for one call");
-    LogitsArgs a = {*r, (char *)out, (const char *)logits, stride, rows, V, 0};
+    LogitsArgs a = {*r, (char *)out, (const char *)logits, stride, rows, V, 0, 0};
     if (type == BMB_F32)
         launch_logits<float>(a, stream);
     else if (type == BMB_F16)

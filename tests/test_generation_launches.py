@@ -1,0 +1,88 @@
+"""What the generation entry points queue for their largest calls, on the host:
+a small program loads the library and stands in for the HIP calls that launch a
+kernel, so nothing runs and every pointer is a number. A dispatch holds fewer
+than 2^32 lanes: larger work has to come in several."""
+import os
+import subprocess
+
+import pytest
+
+import bmb
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include <dlfcn.h>
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+#include "flash.h"
+#include "nn.h"
+typedef struct { unsigned x, y, z; } dim3;
+static dim3 grid, block;
+int __hipPushCallConfiguration(dim3 g, dim3 b, size_t lds, void *stream) {
+    grid = g, block = b;
+    return 0;
+}
+int __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *lds, void **stream) {
+    *g = grid, *b = block, *lds = 0, *stream = 0;
+    return 0;
+}
+int hipLaunchKernel(const void *f, dim3 g, dim3 b, void **args, size_t lds, void *stream) {
+    printf("launch %u %u\n", g.x * g.y * g.z, b.x);
+    return 0;
+}
+int hipGetLastError(void) { return 0; }
+int hipGetDevice(int *d) { *d = 0; return 0; }
+int hipFuncSetAttribute(const void *f, int what, int value) { return 0; }
+static void *at(long long n) { return (void *)(n << 20); }
+int main(int argc, char **argv) {
+    void *lib = dlopen(argv[1], RTLD_NOW);
+    if (!lib) { fprintf(stderr, "%s\n", dlerror()); return 2; }
+    const char *what = argv[2];
+    long long n[8] = {0};
+    for (int i = 3; i < argc; ++i) n[i - 3] = atoll(argv[i]);
+    int rc = 2;
+    if (!strcmp(what, "logits")) {  /* type, rows, V */
+        int (*f)(void *, const void *, int, int, int, long long, const LogitsRules *, void *) =
+            dlsym(lib, "logits_process");
+        LogitsRules r = {0};
+        rc = f(at(1), at(1), n[0], n[1], n[2], n[2], &r, 0);
+    }
+    printf("end %d\n", rc);
+    return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def program(tmp_path_factory):
+    d = tmp_path_factory.mktemp("launches")
+    src, exe = d / "p.c", d / "p"
+    src.write_text(PROGRAM)
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-rdynamic", "-I",
+                    os.path.join(ROOT, "include"), str(src), "-o", str(exe), "-ldl"], check=True)
+    return str(exe)
+
+
+def launches(program, what, *args):
+    """(workgroups, lanes of one) of each launch of a call that is accepted."""
+    r = subprocess.run([program, bmb.LIB_PATH, what] + [str(a) for a in args],
+                       capture_output=True, text=True, timeout=60)
+    lines = r.stdout.split("\n")[:-1]
+    assert r.returncode == 0 and lines[-1] == "end 0", (r.stdout, r.stderr)
+    return [tuple(int(x) for x in line.split()[1:]) for line in lines[:-1]]
+
+
+def covered(got, workgroups):
+    assert all(blocks * lanes < 1 << 32 for blocks, lanes in got), got
+    assert sum(blocks for blocks, _ in got) == workgroups, got
+
+
+@pytest.mark.parametrize("type,ids", [(bmb.F32, 2048), (bmb.F16, 2048), (bmb.BF16, 2048)])
+@pytest.mark.parametrize("rows,V", [(4, 50257), ((1 << 24) - 1, 65), (1 << 24, 65),
+                                    ((1 << 24) + 5, 65), (1 << 26, 4096), ((1 << 31) - 1, 1)])
+def test_logits(program, type, ids, rows, V):
+    few = rows * V < 512 * ids and type == bmb.F32
+    chunks = -(-V // (ids // 2 if few else ids))
+    covered(launches(program, "logits", type, rows, V), rows * chunks)

@@ -211,6 +211,33 @@ def test_logits_offsets_past_32_bits(gpu):
     assert (out[-1, :-1] == 2.0).all() and out[-1, -1] == 1.0 and (out[:-1] == 0).all()
 
 
+def test_logits_rows_of_several_launches(gpu):
+    """More rows than one dispatch has lanes for: every row follows its rules."""
+    rows, V = (1 << 24) + 5, 65
+    x = torch.full((rows, V), 4.0, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros_like(x)
+    row = torch.arange(rows, device="cuda")
+    tok = (row * 7 % V).to(torch.int32)
+    lens = torch.ones(rows, dtype=torch.int32, device="cuda")
+    rep = (1 + row % 2).float()                                   # 1 or 2
+    offsets = torch.arange(rows + 1, device="cuda", dtype=torch.int32)
+    ids, values = ((tok + 1) % V).to(torch.int32), (row % 5).float()
+    words = torch.tensor([~(1 << 3), -1, -1], dtype=torch.int32, device="cuda")
+    index = torch.where(row % 3 == 0, 0, -1).to(torch.int32)
+    rules = bmb.LogitsRules(tokens=tok.data_ptr(), token_stride=1, lens=lens.data_ptr(),
+                            repetition=rep.data_ptr(), bias_offsets=offsets.data_ptr(),
+                            bias_ids=ids.data_ptr(), bias_values=values.data_ptr(), biases=rows,
+                            mask=words.data_ptr(), masks=1, mask_stride=3,
+                            mask_index=index.data_ptr())
+    bmb.logits_process(out.data_ptr(), x.data_ptr(), bmb.BF16, rows, V, V, rules)
+    torch.cuda.synchronize()
+    bmb.check("logits_process")
+    x.scatter_(1, tok[:, None].long(), (4.0 / rep).to(x.dtype)[:, None])
+    x.scatter_add_(1, ids[:, None].long(), values.to(x.dtype)[:, None])
+    x[:, 3] = torch.where(row % 3 == 0, -math.inf, x[:, 3])
+    assert torch.equal(out, x)
+
+
 def test_logits_captured(gpu):
     """Captured on a side stream and replayed on changed inputs."""
     c = Case(8, 5003, "bf16", None, seed=9)
