@@ -193,6 +193,7 @@ struct AppendArgs {
     const int *slots;
     long long row_stride, page_stride, token_stride, head_stride;  // elements
     long long items;   // 8-element pieces of one half
+    long long first;   // the launch's first workgroup of the call's
     int capacity;      // slots of the cache
     FastDiv page, heads;
     int page_size, kv_heads;
@@ -209,7 +210,7 @@ using Vec8 __attribute__((ext_vector_type(8))) = T;
 template <typename TS, typename TC, int HS>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr int PIECES = HS / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long i = (a.first + blockIdx.x) * 256 + threadIdx.x;
     if (i >= a.items) return;
     const int piece = (int)(i % PIECES), row = (int)(i / PIECES);  // row: (token, head)
     const int token = a.heads.quot(row), head = row - token * a.kv_heads;
@@ -227,14 +228,14 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 }
 
 template <typename TS, typename TC>
-void launch_append(int hs, const AppendArgs &a, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.items + 255) / 256)), block(256);
-    if (hs == 32)
-        launch(append_kernel<TS, TC, 32>, grid, block, 0, stream, a);
-    else if (hs == 64)
-        launch(append_kernel<TS, TC, 64>, grid, block, 0, stream, a);
-    else
-        launch(append_kernel<TS, TC, 128>, grid, block, 0, stream, a);
+void launch_append(int hs, AppendArgs &a, hipStream_t stream) {
+    const auto kernel = hs == 32   ? append_kernel<TS, TC, 32>
+                        : hs == 64 ? append_kernel<TS, TC, 64>
+                                   : append_kernel<TS, TC, 128>;
+    in_launches((a.items + 255) / 256, 256, [&](long long first, unsigned n) {
+        a.first = first;
+        launch(kernel, dim3(n), dim3(256), 0, stream, a);
+    });
 }
 
 }  // namespace
@@ -306,7 +307,7 @@ int paged_append(const PagedCache *c, const void *k, const void *v, int type, lo
         return refuse(me, "rows are no multiples of 4 bytes");
     AppendArgs a = {(const char *)k, (const char *)v, (char *)c->k, (char *)c->v, slots, row_stride,
                     c->page_stride, c->token_stride, c->head_stride,
-                    (long long)tokens * c->kv_heads * (c->head_size / 8),
+                    (long long)tokens * c->kv_heads * (c->head_size / 8), 0,
                     c->pages * c->page_size, FastDiv::of(c->page_size), FastDiv::of(c->kv_heads),
                     c->page_size, c->kv_heads};
     const int hs = c->head_size;

@@ -49,6 +49,12 @@ int main(int argc, char **argv) {
         LogitsRules r = {0};
         rc = f(at(1), at(1), n[0], n[1], n[2], n[2], &r, 0);
     }
+    if (!strcmp(what, "append")) {  /* type, cache's type, kv, hs, tokens */
+        int (*f)(const PagedCache *, const void *, const void *, int, long long, const int *, int,
+                 void *) = dlsym(lib, "paged_append");
+        PagedCache c = {at(1), at(2), n[1], 8, 16, n[2], n[3], 16 * n[2] * n[3], n[2] * n[3], n[3]};
+        rc = f(&c, at(3), at(4), n[0], 0, at(5), n[4], 0);
+    }
     printf("end %d\n", rc);
     return 0;
 }
@@ -86,3 +92,13 @@ def test_logits(program, type, ids, rows, V):
     few = rows * V < 512 * ids and type == bmb.F32
     chunks = -(-V // (ids // 2 if few else ids))
     covered(launches(program, "logits", type, rows, V), rows * chunks)
+
+
+@pytest.mark.parametrize("type,cache", [(bmb.F32, bmb.F32), (bmb.F32, bmb.F16),
+                                        (bmb.F32, bmb.BF16), (bmb.F16, bmb.F16)])
+@pytest.mark.parametrize("kv,hs,tokens", [(1, 32, 1), (12, 64, 32), (8, 128, (1 << 25) - 1),
+                                          (8, 128, 1 << 25), (1, 64, (1 << 29) + 9),
+                                          (3, 32, (1 << 29) + 1), (1, 128, (1 << 31) - 1)])
+def test_append(program, type, cache, kv, hs, tokens):
+    covered(launches(program, "append", type, cache, kv, hs, tokens),
+            -(-tokens * kv * hs // 8 // 256))

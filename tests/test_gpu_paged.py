@@ -179,6 +179,29 @@ def test_append(gpu, type, cache, tokens, kv, hs, page, layout):
         assert same.all()
 
 
+def test_append_tokens_of_several_launches(gpu):
+    """More elements than one dispatch has lanes for: the tokens with a slot, at
+    both ends and around where a launch ends, arrive; nothing else is written."""
+    kv, hs, page, tokens = 8, 128, 4, (1 << 25) + 3
+    ends = ((1 << 32) - 1) // 256 // 8 * 8 * 256 // (kv * hs // 8)
+    live = [0, 1, ends - 1, ends, ends + 1, (1 << 25) - 1, 1 << 25, tokens - 1]
+    # rows one element apart: row t is elements t..t+1023
+    rows = torch.randn(2, tokens + kv * hs, device="cuda")
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")
+    at = [2 * i + 1 for i in range(len(live))]
+    slots[torch.tensor(live, device="cuda")] = ints(at)
+    k = torch.full((5, page, kv, hs), 768.0, device="cuda")
+    v = k.clone()
+    want_k, want_v = k.clone().view(-1, kv * hs), v.clone().view(-1, kv * hs)
+    for t, s in zip(live, at):
+        want_k[s], want_v[s] = rows[0, t:t + kv * hs], rows[1, t:t + kv * hs]
+    bmb.paged_append(cache_struct(k, v, "token", page, kv, hs, "f32"), rows[0].data_ptr(),
+                     rows[1].data_ptr(), bmb.F32, 1, slots.data_ptr(), tokens)
+    torch.cuda.synchronize()
+    bmb.check("paged_append")
+    assert torch.equal(k.view(-1, kv * hs), want_k) and torch.equal(v.view(-1, kv * hs), want_v)
+
+
 # -------------------------------------------------------------- attention
 @pytest.mark.parametrize("type,cache", TYPES)
 @pytest.mark.parametrize("hs", [32, 64, 128])
