@@ -57,6 +57,7 @@ struct AttendArgs {
     int few;            // parts that give each CU a workgroup
     int least, enough;  // units of a part: at least; more than `enough` only past `few` parts
     int cached;         // units that stay in the caches; without workers: whether they do
+    int first;          // the launch's first workgroup of the call's
     float scale;        // times log2(e)
     FastDiv page;
     uint32_t page16, token16;  // strides in units of 16 bytes
@@ -556,8 +557,8 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
 
     // Workgroups go to the XCDs in turn: all heads of a slot on one of them,
     // since rows of neighbouring heads can share cache lines.
-    const int per = 8 * a.kv_heads * a.tiles;
-    const int in = blockIdx.x % per, slot = blockIdx.x / per * 8 + in % 8;
+    const uint32_t per = 8 * a.kv_heads * a.tiles, block = a.first + blockIdx.x;
+    const int in = block % per, slot = block / per * 8 + in % 8;
     if (slot >= a.slots) return;
     const int kv_head = in / 8 / a.tiles, tile = in / 8 % a.tiles;
     const Part part = find_part(a, slot);
@@ -788,8 +789,8 @@ __global__ __launch_bounds__(WAVES *WAVE) void attend_rows_kernel(AttendArgs a) 
     float(*part_ml)[2][G] = (float(*)[2][G])merge;
     float *part_o = merge + WAVES * 2 * G;  // (wave, head, element)
 
-    const int per = 8 * a.kv_heads * a.tiles;
-    const int in = blockIdx.x % per, slot = blockIdx.x / per * 8 + in % 8;
+    const uint32_t per = 8 * a.kv_heads * a.tiles, block = a.first + blockIdx.x;
+    const int in = block % per, slot = block / per * 8 + in % 8;
     if (slot >= a.slots) return;
     const int kv_head = in / 8 / a.tiles, tile = in / 8 % a.tiles;
     const Part part = find_part(a, slot);
@@ -860,7 +861,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(AttendArgs a) {
     constexpr int LANES = HS / 4, SHARES = JOIN_THREADS / LANES;
     __shared__ float4 acc_s[SHARES][LANES];
     __shared__ float sum_s[SHARES], top_s[SHARES];
-    const int r = blockIdx.x / a.heads, head = blockIdx.x % a.heads, tid = threadIdx.x;
+    const uint32_t block = a.first + blockIdx.x;
+    const int r = block / a.heads, head = block % a.heads, tid = threadIdx.x;
     const int row = row_of(a, r), len = len_of(a, r);
     const int4 parts = a.parts[r];
     const int n = parts.y + (parts.z >= 0);
@@ -1002,13 +1004,22 @@ const char *batch_fault(const PagedCache *c, const PagedBatch *b) {
     return nullptr;
 }
 
-// One launch of `kernel`, whose workgroups of `waves` waves take `cols` heads each.
+// `blocks` workgroups of `kernel`.
+void launch_blocks(void (*kernel)(AttendArgs), long long blocks, int threads, size_t lds,
+                   AttendArgs a, hipStream_t stream) {
+    in_launches(blocks, threads, [&](long long first, unsigned n) {
+        a.first = (int)first;
+        launch(kernel, dim3(n), dim3(threads), lds, stream, a);
+    });
+}
+
+// The parts by `kernel`, whose workgroups of `waves` waves take `cols` heads each.
 void launch_parts(void (*kernel)(AttendArgs), int waves, int cols, int hs, const AttendArgs &a,
                   hipStream_t stream) {
-    const dim3 grid((unsigned)((a.slots + 7) / 8 * 8 * a.kv_heads * a.tiles)), block(waves * WAVE);
     const size_t lds = merge_bytes(waves, cols, a.group < cols ? a.group : cols, hs);
     allow_smem(kernel, lds);
-    launch(kernel, grid, block, lds, stream, a);
+    launch_blocks(kernel, (a.slots + 7ll) / 8 * 8 * a.kv_heads * a.tiles, waves * WAVE, lds, a,
+                  stream);
 }
 
 template <template <typename, int> class POLICY, typename TC, int HS, int QT>
@@ -1052,8 +1063,8 @@ void launch_attend(const AttendArgs &a, hipStream_t stream) {
             launch_matrix<Full, TC, HS, 1>(a, stream);
     }
     if (a.workers)
-        launch(join_kernel<TQ, HS>, dim3((unsigned)(a.requests * a.heads)), dim3(JOIN_THREADS), 0,
-               stream, a);
+        launch_blocks(join_kernel<TQ, HS>, (long long)a.requests * a.heads, JOIN_THREADS, 0, a,
+                      stream);
 }
 
 template <typename TQ, typename TC>
@@ -1108,7 +1119,7 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
                     (int4 *)(work + s.parts_at), c->page_stride, c->token_stride, c->head_stride,
                     b->q_stride, b->out_stride, b->requests, b->heads, c->kv_heads, group,
                     tiles_of(*c, *b), c->pages, b->table_stride, b->max_len, b->n_rows,
-                    s.slots, s.workers, s.few, s.least, s.enough, s.cached, b->scale * LOG2E,
+                    s.slots, s.workers, s.few, s.least, s.enough, s.cached, 0, b->scale * LOG2E,
                     FastDiv::of(c->page_size),
                     (uint32_t)(c->page_stride * size / 16),
                     (uint32_t)(c->token_stride * size / 16)};

@@ -55,6 +55,15 @@ int main(int argc, char **argv) {
         PagedCache c = {at(1), at(2), n[1], 8, 16, n[2], n[3], 16 * n[2] * n[3], n[2] * n[3], n[3]};
         rc = f(&c, at(3), at(4), n[0], 0, at(5), n[4], 0);
     }
+    if (!strcmp(what, "attend")) {  /* type, cache's type, hs, heads, kv, requests, max_len */
+        int (*f)(const PagedCache *, const PagedBatch *, void *, float *, const void *, void *) =
+            dlsym(lib, "paged_attention");
+        PagedCache c = {at(1), at(2), n[1], 1, 1 << 24, n[4], n[2], 0, n[2] * n[4], n[2]};
+        PagedBatch b = {n[5], n[6], 1, n[3], n[5], n[0], 1.0f, 0, n[2] * n[3]};
+        b.block_table = b.lens = at(3);
+        b.work = at(4), b.work_bytes = ~0ull;
+        rc = f(&c, &b, at(5), 0, at(6), 0);
+    }
     printf("end %d\n", rc);
     return 0;
 }
@@ -102,3 +111,30 @@ def test_logits(program, type, ids, rows, V):
 def test_append(program, type, cache, kv, hs, tokens):
     covered(launches(program, "append", type, cache, kv, hs, tokens),
             -(-tokens * kv * hs // 8 // 256))
+
+
+@pytest.mark.parametrize("type,cache", [(bmb.F32, bmb.F32), (bmb.F32, bmb.BF16),
+                                        (bmb.F16, bmb.F16)])
+@pytest.mark.parametrize("heads,kv", [(32, 32), (64, 16), (66, 2), (256, 8)])
+@pytest.mark.parametrize("requests,split", [(3, False), (3, True), ((1 << 18) + 1, False),
+                                            (1 << 19, False), ((1 << 19) + 9, False),
+                                            ((1 << 23) + 1, False)])
+def test_attention(program, type, cache, heads, kv, requests, split):
+    if heads > 64 and requests > 1 << 20:
+        requests = 1 << 22
+    tiles = -(-heads // kv // (32 if type != bmb.F32 and heads // kv > 16 else 16))
+    blocks = -(-(requests + split * (2048 // (kv * tiles))) // 8) * 8 * kv * tiles
+    got = launches(program, "attend", type, cache, 32, heads, kv, requests,
+                   1 << 20 if split else 3)
+    covered(got, blocks + split * requests * heads)
+
+
+@pytest.mark.parametrize("type,cache", [(bmb.F32, bmb.F32), (bmb.F16, bmb.F16)])
+@pytest.mark.parametrize("requests", [(1 << 11) - 1, 1 << 11, (1 << 11) + 1])
+def test_attention_joins(program, type, cache, requests):
+    """Split sequences: as many joins as a dispatch has lanes for, and more."""
+    heads, kv, max_len = 1 << 13, 256, 1 << 23
+    tiles = 1 if type == bmb.F16 else 2
+    blocks = -(-(requests + 2048 // (kv * tiles)) // 8) * 8 * kv * tiles
+    covered(launches(program, "attend", type, cache, 32, heads, kv, requests, max_len),
+            blocks + requests * heads)

@@ -435,6 +435,80 @@ def test_attention_offsets_past_32_bits(gpu, page):
     assert torch.equal(v[0, 5].view(-1), rows[1, kv * hs:])
 
 
+@pytest.mark.parametrize("type,cache,heads", [("f32", "f32", 32), ("f16", "f16", 64)])
+def test_attention_parts_of_several_launches(gpu, type, cache, heads):
+    """More requests than one dispatch has lanes for: the bits of a few of them
+    alone, over and over."""
+    kv, hs, few = 32, 32, 61
+    small = Problem([i % 4 for i in range(few)], heads, kv, hs, type, cache, 16, seed=23)
+    d = small.device()
+    d.run()
+    d.check()
+    requests, W = (1 << 19) + 11, heads * hs
+    times = -(-requests // few)
+    table, lens, q = (x.repeat(times, *[1] * (x.dim() - 1))[:requests].contiguous()
+                      for x in (d.table, d.lens, d.q[:, :W]))
+    out = torch.full((requests, W), 768.0, dtype=DTYPES[type], device="cuda")
+    lse = torch.full((requests, heads), 768.0, device="cuda")
+    b = d.batch
+    b.requests = b.n_rows = requests
+    b.q_stride = b.out_stride = W
+    b.block_table, b.lens = table.data_ptr(), lens.data_ptr()
+    assert bmb.paged_attention_workspace(d.cache, b) == 0
+    bmb.paged_attention(d.cache, b, out.data_ptr(), lse.data_ptr(), q.data_ptr())
+    torch.cuda.synchronize()
+    bmb.check("paged_attention")
+    for got, want in ((out, d.out[:, :W]), (lse, d.lse)):
+        whole = requests // few * few
+        assert (got[:whole].view(-1, *want.shape) == want).all()
+        assert torch.equal(got[whole:], want[:requests - whole])
+
+
+def test_attention_joins_of_several_launches(gpu):
+    """More heads of requests than one dispatch has lanes for, the last request
+    split: its joined rows within the bound, every other the one value it has."""
+    requests, heads, kv, hs, page, n = 2051, 8192, 256, 32, 4096, 100000
+    pages, max_len, G, W = pages_of(n, page), 1 << 21, heads // kv, heads * hs
+    g = torch.Generator(device="cuda").manual_seed(24)
+    k, v = (torch.empty(pages, page, kv, hs, device="cuda", dtype=torch.float16)
+            .normal_(generator=g) for _ in range(2))
+    q = torch.empty(W, device="cuda", dtype=torch.float16).normal_(generator=g)
+    table = torch.zeros(requests, pages_of(max_len, page) + 1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(requests, device="cuda") % pages
+    table[-1, :pages] = torch.arange(pages, device="cuda")
+    lens = torch.ones(requests, dtype=torch.int32, device="cuda")
+    lens[-1] = n
+    out = torch.full((requests, W), 768.0, dtype=torch.float16, device="cuda")
+    batch = bmb.PagedBatch(requests=requests, max_len=max_len + 1, table_stride=table.shape[1],
+                           heads=heads, n_rows=requests, type=bmb.F16, scale=1 / math.sqrt(hs),
+                           q_stride=0, out_stride=W, block_table=table.data_ptr(),
+                           lens=lens.data_ptr())
+    cache = cache_struct(k, v, "token", page, kv, hs, "f16")
+    need = bmb.paged_attention_workspace(cache, batch)
+    assert need > 0 and requests * heads * 256 > 1 << 32
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    batch.work, batch.work_bytes = work.data_ptr(), need
+    bmb.paged_attention(cache, batch, out.data_ptr(), None, q.data_ptr())
+    torch.cuda.synchronize()
+    bmb.check("paged_attention")
+    for p in range(pages):  # one key: its value
+        assert (out[p:-1:pages].view(-1, kv, G, hs) == v[p, 0][:, None]).all()
+    for h in (0, 100, kv - 1):
+        x = (q.view(kv, G, hs)[h].double() @ k.view(-1, kv, hs)[:n, h].double().t()) / math.sqrt(hs)
+        values = v.view(-1, kv, hs)[:n, h].double()
+        weights = torch.softmax(x, 1)
+        want = weights @ values
+        # as Problem.exact
+        mag = (q.view(kv, G, hs)[h].abs().double()
+               @ k.view(-1, kv, hs)[:n, h].abs().double().t()).amax(1) / math.sqrt(hs)
+        eps = (2 * (4 * (math.sqrt(hs) + 1) * U32 * mag + 4 * U32 * x.abs().amax(1))
+               + (4 * math.sqrt(n) + 16) * U32 + 2.0 ** -23)
+        bound = (eps[:, None] * (weights @ values.abs()) + 2.0 ** -40 * values.abs().sum(0)
+                 + 2.0 ** -11 * want.abs() + 2.0 ** -25)
+        got = out[-1].view(kv, G, hs)[h].double()
+        assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max()
+
+
 def test_attention_streams_and_scratch(gpu):
     """Leased scratch on two streams in turn, and the same bits as with a
     workspace of the caller's, every time."""
