@@ -111,10 +111,11 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
     __syncthreads();
     if (counts) {
         const int *tokens = r.tokens + row * r.token_stride;
-        const int len = (int)min((long long)max(r.lens[row], 0), r.token_stride);
-        const int prompt = r.prompt_lens ? r.prompt_lens[row] : 0;
+        // (32 unsigned bits: steps behind the end of up to 2^31 - 1 tokens)
+        const uint32_t len = (uint32_t)min((long long)max(r.lens[row], 0), r.token_stride);
+        const uint32_t prompt = r.prompt_lens ? max(r.prompt_lens[row], 0) : 0;
         constexpr int AHEAD = 4;  // loads in flight
-        for (int base = tid; base < len; base += AHEAD * THREADS) {
+        for (uint32_t base = tid; base < len; base += AHEAD * THREADS) {
             int id[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
@@ -129,9 +130,9 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
             }
         }
     }
-    for (int i = b0 + tid; i < b1; i += THREADS) {
+    for (uint32_t i = b0 + tid; i < (uint32_t)b1; i += THREADS) {
         const int id = r.bias_ids[i];
-        if (id >= lo && id < hi) atomicMax(&bias[id + word], (uint32_t)(i - b0) + 1);
+        if (id >= lo && id < hi) atomicMax(&bias[id + word], i - b0 + 1);
     }
     __syncthreads();
 

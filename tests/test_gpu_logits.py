@@ -238,6 +238,43 @@ def test_logits_rows_of_several_launches(gpu):
     assert torch.equal(out, x)
 
 
+def test_logits_longest_history(gpu):
+    """2^31 - 1 tokens, the most that a length can say, the last two of them the
+    only ones of the vocabulary."""
+    n, V = (1 << 31) - 1, 70
+    tokens = torch.full((1, n), -1, dtype=torch.int32, device="cuda")
+    tokens[0, -2:] = ints = i32([7, 69])
+    x = torch.full((1, V), 8.0, device="cuda")
+    out = torch.zeros_like(x)
+    lens, prompt = i32([n]), i32([n - 1])
+    rep, freq = torch.full((1,), 2.0, device="cuda"), torch.full((1,), 0.5, device="cuda")
+    rules = bmb.LogitsRules(tokens=tokens.data_ptr(), token_stride=n, lens=lens.data_ptr(),
+                            prompt_lens=prompt.data_ptr(), repetition=rep.data_ptr(),
+                            frequency=freq.data_ptr())
+    bmb.logits_process(out.data_ptr(), x.data_ptr(), bmb.F32, 1, V, V, rules)
+    torch.cuda.synchronize()
+    bmb.check("logits_process")
+    x[0, ints.long()] = torch.tensor([4.0, 3.5], device="cuda")
+    assert torch.equal(out, x)
+
+
+def test_logits_biases_at_the_largest_offsets(gpu):
+    """A row's entries at the end of a list of 2^31 - 1, of which only they exist."""
+    n, V = 700, 90
+    b1 = (1 << 31) - 1
+    b0 = b1 - n
+    ids = torch.arange(n, device="cuda", dtype=torch.int32) % 100
+    values = torch.arange(n, device="cuda").float()
+    offsets = i32([b0, b1])
+    x, out = torch.zeros(1, V, device="cuda"), torch.ones(1, V, device="cuda")
+    rules = bmb.LogitsRules(bias_offsets=offsets.data_ptr(), bias_ids=ids.data_ptr() - 4 * b0,
+                            bias_values=values.data_ptr() - 4 * b0, biases=b1)
+    bmb.logits_process(out.data_ptr(), x.data_ptr(), bmb.F32, 1, V, V, rules)
+    torch.cuda.synchronize()
+    bmb.check("logits_process")
+    assert out[0].tolist() == [600.0 + i for i in range(V)]  # the last entry of each id
+
+
 def test_logits_captured(gpu):
     """Captured on a side stream and replayed on changed inputs."""
     c = Case(8, 5003, "bf16", None, seed=9)
