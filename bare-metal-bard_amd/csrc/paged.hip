@@ -293,7 +293,7 @@ int paged_append(const PagedCache *c, const void *k, const void *v, int type, lo
                  const int *slots, int tokens, hipStream_t stream) {
     using namespace bmb;
     const char *me = "paged_append";
-    if (const char *why = cache_fault(c)) return refuse(me, why);
+    if (const char *why = cache_fault(c, true)) return refuse(me, why);
     const int size = element_size(type);
     if (size == 0) return refuse(me, "unknown element type");
     if (type != BMB_F32 && type != c->type)

@@ -63,18 +63,17 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 }
 
 // The cache's own description, checked: nullptr if a call may use it, else why
-// not.
-inline const char *cache_fault(const PagedCache *c) {
-    if (c == nullptr || c->k == nullptr || c->v == nullptr) return "no cache";
+// not. Without `buffers` its pointers are not looked at.
+inline const char *cache_fault(const PagedCache *c, bool buffers) {
+    if (c == nullptr || (buffers && (c->k == nullptr || c->v == nullptr))) return "no cache";
     const int size = element_size(c->type);
     if (size == 0) return "unknown element type of the cache";
     if (c->pages < 1 || c->page_size < 1 || c->kv_heads < 1) return "empty cache";
     if (c->head_size != 32 && c->head_size != 64 && c->head_size != 128)
         return "head size is not 32, 64 or 128";
     if ((long long)c->pages * c->page_size > INT_MAX) return "2^31 or more tokens in the cache";
-    const unsigned long long bits = (unsigned long long)(uintptr_t)c->k |
-                                    (unsigned long long)(uintptr_t)c->v |
-                                    (unsigned long long)(c->page_stride * size) |
+    const unsigned long long halves = buffers ? (uintptr_t)c->k | (uintptr_t)c->v : 0;
+    const unsigned long long bits = halves | (unsigned long long)(c->page_stride * size) |
                                     (unsigned long long)(c->token_stride * size) |
                                     (unsigned long long)(c->head_stride * size);
     if (bits % 16 != 0) return "the cache's buffers and strides are no multiples of 16 bytes";

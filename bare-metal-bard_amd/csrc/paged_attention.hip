@@ -980,8 +980,9 @@ Split split_of(const PagedCache &c, const PagedBatch &b) {
     return s;
 }
 
-const char *batch_fault(const PagedCache *c, const PagedBatch *b) {
-    if (const char *why = cache_fault(c)) return why;
+// (`buffers`: as for cache_fault.)
+const char *batch_fault(const PagedCache *c, const PagedBatch *b, bool buffers) {
+    if (const char *why = cache_fault(c, buffers)) return why;
     if (b == nullptr) return "no batch";
     if (b->requests < 1 || b->max_len < 0 || b->heads < 1 || b->n_rows < 1)
         return "a size is below its least";
@@ -1083,7 +1084,7 @@ void launch_attend(int hs, const AttendArgs &a, hipStream_t stream) {
 extern "C" {
 
 size_t paged_attention_workspace(const PagedCache *cache, const PagedBatch *batch) {
-    if (bmb::batch_fault(cache, batch)) return 0;
+    if (bmb::batch_fault(cache, batch, false)) return 0;
     return bmb::split_of(*cache, *batch).bytes;
 }
 
@@ -1091,7 +1092,7 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
                     hipStream_t stream) {
     using namespace bmb;
     const char *me = "paged_attention";
-    if (const char *why = batch_fault(c, b)) return refuse(me, why);
+    if (const char *why = batch_fault(c, b, true)) return refuse(me, why);
     if (!out || !q || !b->block_table || !b->lens) return refuse(me, "a null pointer");
     if (((uintptr_t)q | (uintptr_t)out) % 4 != 0)
         return refuse(me, "rows are no multiples of 4 bytes");

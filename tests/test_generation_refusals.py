@@ -141,6 +141,22 @@ def test_attention_refuses_small_workspaces(capfd):
     refused(capfd, "16 bytes", bmb.paged_attention, cache(), b, P, P, P)
 
 
+@pytest.mark.parametrize("kw", [dict(k=None, v=None), dict(k=None), dict(v=None),
+                                dict(k=P + 8), dict(v=P + 4)])
+def test_workspace_looks_at_no_pointer(kw):
+    """Its bytes are known before the cache and the batch have their buffers."""
+    b = batch(max_len=64000, table_stride=4000)
+    need = bmb.paged_attention_workspace(cache(), b)
+    b.block_table = b.lens = None
+    assert need > 0 and bmb.paged_attention_workspace(cache(**kw), b) == need
+    assert bmb.paged_attention_workspace(cache(head_size=48, **kw), b) == 0
+
+
+def test_workspace_of_nothing():
+    assert bmb.paged_attention_workspace(None, batch()) == 0
+    assert bmb.paged_attention_workspace(cache(), None) == 0
+
+
 def rules(**kw):
     f = dict(tokens=P, token_stride=8, lens=P, repetition=P, bias_offsets=P, bias_ids=P,
              bias_values=P, biases=2, mask=P, masks=4, mask_stride=4)
