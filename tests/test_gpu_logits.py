@@ -195,6 +195,36 @@ def test_logits_clipped_device_values(gpu):
     bmb.check("logits_process")
 
 
+def test_logits_clipped_bias_offsets(gpu):
+    """Offsets outside the list are read as its ends, and a range that ends before
+    it begins is empty."""
+    c = Case(6, 500, "f32", biases=0, seed=6)
+    n = 40
+    c.bias_ids = (np.arange(n) * 11) % 250  # each a few times: the last entry counts
+    c.bias = (np.arange(n) + 1).astype(np.float32)
+    c.offsets = np.array([0, 0, 0, 0, 0, 0, n])
+    c.run()
+    given = [-4, 7, 3, -1, 1 << 30, 25, n + 1]
+    clipped = [min(max(x, 0), n) for x in given]
+    off = i32(given)
+    c.rules.bias_offsets = off.data_ptr()
+    bmb.logits_process(*c.args)
+    torch.cuda.synchronize()
+    bmb.check("logits_process")
+    got = c.dst.view(c.rows, c.stride)[:, :c.V].cpu()
+    for r in range(c.rows):
+        b, e = clipped[r], clipped[r + 1]
+        assert (b < e) == (r in (0, 3, 5))
+        c.offsets = np.zeros(c.rows + 1, int)  # of row r alone
+        c.offsets[r], c.offsets[r + 1] = b, max(b, e)
+        want, tol = c.exact(True, True, True)
+        with np.errstate(invalid="ignore"):
+            x = got[r].double().numpy()
+            same = (x == want[r]) | (np.isnan(x) & np.isnan(want[r])) | (
+                np.abs(x - want[r]) <= tol[r] + 2.0 ** -24 * np.abs(want[r]) * (tol[r] > 0))
+        assert same.all(), (r, np.argwhere(~same)[:4])
+
+
 def test_logits_offsets_past_32_bits(gpu):
     """Rows that start more than 2^31 elements into the buffers."""
     V, rows = 1 << 20, 2080
