@@ -230,6 +230,112 @@ def test_attention_split(gpu, type, cache, hs, lens, heads, kv, page):
     p.check()
 
 
+def large_batch(lens, heads, kv, hs, type, cache, page, max_len, seed):
+    """A batch made on the device, run once with leased scratch, and checked for
+    its first and last live requests and heads: Problem.exact's bound, with what
+    flash.h allows a probability's two 16-bit numbers to lose."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    held = [pages_of(n, page) for n in lens]
+    pages, width = sum(held) + 1, pages_of(max_len, page)
+    order = torch.randperm(pages, device="cuda", generator=g)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device="cuda")
+    k = torch.full((pages, page, kv, hs), math.nan, device="cuda", dtype=DTYPES[cache])
+    v, at = torch.full_like(k, math.inf), 0
+    for r, n in enumerate(lens):
+        table[r, :held[r]] = order[at:at + held[r]]
+        at += held[r]
+        t = torch.arange(n, device="cuda")
+        for half in (k, v):
+            half[table[r].long()[t // page], t % page] = torch.empty(
+                n, kv, hs, device="cuda", dtype=half.dtype).normal_(generator=g)
+    R, W, G = len(lens), heads * hs, heads // kv
+    q = torch.empty(R, W, device="cuda", dtype=DTYPES[type]).normal_(generator=g)
+    out, lse = torch.full_like(q, 768.0), torch.full((R, heads), 768.0, device="cuda")
+    d_lens, scale = ints(lens), 1 / math.sqrt(hs)
+    batch = bmb.PagedBatch(requests=R, max_len=max_len, table_stride=width, heads=heads, n_rows=R,
+                           type=bmb.ELEMENT_TYPES[type], scale=scale, q_stride=W, out_stride=W,
+                           block_table=table.data_ptr(), lens=d_lens.data_ptr())
+    handle = cache_struct(k, v, "token", page, kv, hs, cache)
+    bmb.paged_attention(handle, batch, out.data_ptr(), lse.data_ptr(), q.data_ptr())
+    torch.cuda.synchronize()
+    bmb.check("paged_attention")
+    half_step = torch.finfo(DTYPES[type]).eps / 2
+    lost, floor = dict(f32=(0.0, 0.0), f16=(2.0 ** -23, 2.0 ** -40), bf16=(2.0 ** -17, 0.0))[type]
+    live = [r for r, n in enumerate(lens) if n]
+    assert torch.isfinite(out[live].float()).all() and torch.isfinite(lse[live]).all()
+    for r, n in enumerate(lens):
+        if n == 0:
+            assert (out[r] == 0).all() and (lse[r] == -math.inf).all()
+    for r in live[:2] + live[-2:]:
+        n, t = lens[r], torch.arange(lens[r], device="cuda")
+        for h in sorted({0, kv - 1}):
+            keys, values = (x[table[r].long()[t // page], t % page, h].double() for x in (k, v))
+            qh = q[r].view(kv, G, hs)[h].double()
+            x = qh @ keys.t() * scale
+            mag = (qh.abs() @ keys.abs().t()).amax(1) * scale
+            z = torch.logsumexp(x, 1)
+            p = torch.exp(x - z[:, None])
+            want = p @ values
+            ds = 4 * (math.sqrt(hs) + 1) * U32 * mag + 4 * U32 * x.abs().amax(1)
+            eps = 2 * ds + (4 * math.sqrt(n) + 16) * U32 + lost
+            bound = (eps[:, None] * (p @ values.abs()) + floor * values.abs().sum(0)
+                     + half_step * want.abs() + (2.0 ** -25 if type == "f16" else 0.0))
+            got = out[r].view(kv, G, hs)[h].double()
+            assert ((got - want).abs() <= bound).all(), (r, h, ((got - want).abs() / bound).max())
+            zb = ds + (4 * math.sqrt(n) + 16) * U32 + 4 * U32 * z.abs()
+            assert ((lse[r].view(kv, G)[h].double() - z).abs() <= zb).all(), (r, h)
+    return handle, batch
+
+
+# Batches whose keys and values pass what stays in the caches (1.2e8 bytes), by 128 keys:
+# their loads are non-temporal ones.
+PAST_CACHES = 1.2e8
+
+
+@pytest.mark.parametrize("type,cache", TYPES)
+@pytest.mark.parametrize("hs", [32, 64, 128])
+@pytest.mark.parametrize("group", [1, 3, 5, 20])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attention_split_past_the_caches(gpu, type, cache, hs, group, page):
+    kv = 1024 // hs
+    if type == "f32" and group == 20:
+        group = 16  # (more take two workgroups, which keep the rows for each other)
+    lens = [8300, 1, 8129] if cache == "f32" else [8300, 129, 8129, 0, 8200, 8300]
+    size = DTYPES[cache].itemsize
+    assert sum(lens) * 2 * 1024 * size > PAST_CACHES
+    print("past the caches", type, cache, hs, group, page, flush=True)
+    handle, batch = large_batch(lens, kv * group, kv, hs, type, cache, page, max(lens), seed=hs)
+    assert bmb.paged_attention_workspace(handle, batch) > 0
+
+
+@pytest.mark.parametrize("type,cache", TYPES)
+@pytest.mark.parametrize("hs", [32, 64, 128])
+@pytest.mark.parametrize("group", [1, 5])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attention_whole_past_the_caches(gpu, type, cache, hs, group, page):
+    """The same loads for sequences of one part each."""
+    kv, size = 1024 // hs, DTYPES[cache].itemsize
+    max_len = (512 << 10) // (2 * hs * size)
+    lens = [max_len, 1, 0] + [(37 * i) % max_len for i in range(60)] + [max_len - 1]
+    assert 0.5 * len(lens) * max_len * 2 * 1024 * size > PAST_CACHES
+    handle, batch = large_batch(lens, kv * group, kv, hs, type, cache, page, max_len, seed=hs + 1)
+    assert bmb.paged_attention_workspace(handle, batch) == 0
+
+
+@pytest.mark.parametrize("type,cache,heads", [("bf16", "bf16", 2), ("f32", "f16", 1)])
+@pytest.mark.parametrize("requests", [4097, 4300])
+def test_attention_split_of_thousands_of_requests(gpu, type, cache, heads, requests):
+    """More than 64 requests to a lane of the search for a part: every request's
+    rows, those of the long ones in two of them included."""
+    lens = [i % 3 for i in range(requests)]
+    share = -(-requests // 64)
+    lens[10 * share + share - 1], lens[-1], lens[20 * share] = 9000, 700, 20000
+    d = Problem(lens, heads, 1, 32, type, cache, 16, seed=requests).device()
+    assert share > 64 and d.workspace() > 0
+    d.run()
+    d.check()
+
+
 @pytest.mark.parametrize("type,cache", [("f32", "f32"), ("f16", "f16")])
 def test_attention_many_requests(gpu, type, cache):
     """More workgroups than the device holds at once, every request whole."""
