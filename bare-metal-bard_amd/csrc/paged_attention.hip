@@ -1099,8 +1099,8 @@ int paged_attention(const PagedCache *c, const PagedBatch *b, void *out, float *
     const int size = element_size(c->type);
     if (c->page_size % 16 != 0 &&
         ((c->pages - 1) * c->page_stride + (c->page_size - 1) * c->token_stride) * size / 16 >=
-            0xffffffffll)
-        return refuse(me, "a cache of 64 GiB or more needs pages of a multiple of 16 tokens");
+            NO_ROW)
+        return refuse(me, "tokens 64 GiB apart need pages of a multiple of 16 tokens");
     const Split s = split_of(*c, *b);
     char *work = (char *)b->work;
     if (work != nullptr && b->work_bytes < s.bytes) return refuse(me, "the workspace is too small");

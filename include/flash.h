@@ -112,8 +112,9 @@ bool flash_attention_backward_cfg(int cfg, float *dqkv, float *dsum,
 /* Keys and values of one layer. Element (page, token, head, d) of either half
  * is at page*page_stride + token*token_stride + head*head_stride + d, in
  * elements; buffers and strides are multiples of 16 bytes. head_size: 32, 64
- * or 128. pages * page_size < 2^31, token_stride < 2^26. (Pages of a multiple of 16 tokens are read
- * fastest; paged_attention refuses others in a cache of 64 GiB a half.) */
+ * or 128. pages * page_size < 2^31, token_stride < 2^26. (Pages of a multiple
+ * of 16 tokens are read fastest; paged_attention refuses others where the last
+ * token of the last page starts 64 GiB - 16 bytes or more behind the first.) */
 typedef struct PagedCache {
     void *k, *v;
     int type; /* BMB_F32, BMB_F16 or BMB_BF16 */

@@ -131,6 +131,18 @@ def test_attention_refuses_huge_caches_of_odd_pages(capfd):
     refused(capfd, "64 GiB", bmb.paged_attention, c, batch(table_stride=64), P, P, P)
 
 
+@pytest.mark.parametrize("page_size,last,why", [(24, (1 << 36) - 16, "64 GiB"),
+                                                (24, (1 << 36) - 32, "too small"),
+                                                (32, 1 << 40, "too small")])
+def test_attention_odd_pages_by_their_places(capfd, page_size, last, why):
+    """Not the cache's size: where its last token starts, behind the first. (A
+    workspace that is too small is refused behind that.)"""
+    c = cache(pages=2, page_size=page_size, page_stride=last // 4 - (page_size - 1) * 128)
+    b = batch(max_len=64000, table_stride=4000)
+    b.work, b.work_bytes = P, 16
+    refused(capfd, why, bmb.paged_attention, c, b, P, P, P)
+
+
 def test_attention_refuses_small_workspaces(capfd):
     b = batch(max_len=64000, table_stride=4000)
     need = bmb.paged_attention_workspace(cache(), b)
