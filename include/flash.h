@@ -93,8 +93,8 @@ bool flash_attention_backward_cfg(int cfg, float *dqkv, float *dsum,
  *   paged_plan       once: pages, slots and positions of the step's tokens;
  *   paged_append     per layer: their keys and values into the cache;
  *   paged_attention  per layer: attention of one new token a request.
- * (Prompts attend by flash_attention_forward; append puts their keys and
- * values, which lie in the fused QKV rows, into the cache.)
+ * (Prompts that start a request attend by flash_attention_forward; append puts
+ * their keys and values, which lie in the fused QKV rows, into the cache.)
  *
  * Everything is queued on `stream` of the current device, where all buffers
  * live; results overlap neither inputs nor each other unless said so. Each
@@ -104,10 +104,10 @@ bool flash_attention_backward_cfg(int cfg, float *dqkv, float *dsum,
  * What lies in device memory cannot be refused: lengths are read as if clipped
  * to their range, and page ids, slots and rows outside theirs are skipped. All
  * results depend on the inputs alone (no floating-point atomics; a request's
- * last bits on how its batch is split). Nothing is allocated and nothing
- * outside the given buffers is used, so every call can be captured into a
- * graph (for paged_attention that holds with a workspace of the caller's,
- * below). */
+ * last bits on how its batch is split), but for a slot that is given twice.
+ * Nothing is allocated and nothing outside the given buffers is used, so every
+ * call can be captured into a graph (for paged_attention that holds with a
+ * workspace of the caller's, below). */
 
 /* Keys and values of one layer. Element (page, token, head, d) of either half
  * is at page*page_stride + token*token_stride + head*head_stride + d, in
@@ -162,9 +162,9 @@ int paged_append(const PagedCache *cache, const void *k, const void *v, int type
  * tokens with the query in row rows[r] of q (row r where rows is null); a row
  * outside [0, n_rows) takes no part, and rows of `out` and `lse` that no
  * request names are left as they were. Query head h reads kv head
- * h / (heads / kv_heads). No row is named twice. A row of q and out is heads * head_size elements of
- * `type`: BMB_F32 with a cache of any type, or the cache's own. Rows are
- * multiples of 4 bytes apart.
+ * h / (heads / kv_heads). No row is named twice. A row of q and out is heads *
+ * head_size elements of `type`: BMB_F32 with a cache of any type, or the cache's
+ * own. Rows are multiples of 4 bytes apart.
  *
  * work: device memory of paged_attention_workspace() bytes for the partial
  * results of sequences that are split over their length, used by one call at
