@@ -74,8 +74,9 @@ class GPT(ctypes.Structure):
 
 _GPTP = ctypes.POINTER(GPT)
 
-# Element types of the paged cache and of logits_process (include/flash.h, nn.h).
-F32, F16, BF16 = 0, 1, 2
+# Element types of the paged cache and of nn.h's operators that take one
+# (include/flash.h, nn.h); I8: 8-bit rows with a scale each.
+F32, F16, BF16, I8 = 0, 1, 2, 3
 ELEMENT_TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
 
 
@@ -113,6 +114,41 @@ class LogitsRules(ctypes.Structure):
                    ("mask_index", c_vp)])
 
 
+class RmsNorm(ctypes.Structure):
+    """Mirror of `struct RmsNorm` (include/nn.h); a field left out is null."""
+    _fields_ = ([(n, c_int) for n in ("rows", "C", "type", "out_type")] + [("eps", c_float)]
+                + [(n, c_vp) for n in ("x", "residual", "sum", "weight", "out", "scales", "rstd")]
+                + [(n, c_ll) for n in ("x_stride", "residual_stride", "sum_stride",
+                                       "out_stride")])
+
+
+class RmsNormGrad(ctypes.Structure):
+    """Mirror of `struct RmsNormGrad` (include/nn.h)."""
+    _fields_ = ([(n, c_int) for n in ("rows", "C", "type")]
+                + [(n, c_vp) for n in ("dout", "inp", "dres", "weight", "rstd", "dinp", "dweight")]
+                + [(n, c_ll) for n in ("dout_stride", "inp_stride", "dres_stride", "dinp_stride")]
+                + [("work", c_vp), ("work_bytes", c_size_t)])
+
+
+# include/nn.h
+ROTARY_HALF, ROTARY_PAIRS = 0, 1
+ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_BASE, ROTARY_PARTS = 0, 1, 2, 3
+
+
+class Rotary(ctypes.Structure):
+    """Mirror of `struct Rotary` (include/nn.h)."""
+    _fields_ = [("head_size", c_int), ("dims", c_int), ("layout", c_int), ("amplitude", c_float),
+                ("freq", c_double * 128)]
+
+
+class GemmI8(ctypes.Structure):
+    """Mirror of `struct GemmI8` (include/gemm.h)."""
+    _fields_ = ([(n, c_int) for n in ("M", "N", "K", "type")]
+                + [(n, c_vp) for n in ("A", "B", "a_scales", "b_scales", "bias", "C")]
+                + [(n, c_ll) for n in ("lda", "ldb", "ldc")]
+                + [("work", c_vp), ("work_bytes", c_size_t)])
+
+
 _CACHEP, _BATCHP = ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch)
 
 # Every symbol the C headers declare, with its ctypes signature.
@@ -139,6 +175,8 @@ _SIGS = {
                              c_float, c_vp, c_vp]),
     "gemm_set_math": (c_int, [c_int]),
     "gemm_get_math": (c_int, []),
+    "gemm_i8": (c_int, [ctypes.POINTER(GemmI8), c_vp]),
+    "gemm_i8_workspace": (c_size_t, [ctypes.POINTER(GemmI8)]),
     # flash.h
     "flash_attention_forward": (None, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int]),
     "flash_attention_backward": (None, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int,
@@ -183,6 +221,16 @@ _SIGS = {
     "reduce_mean": (c_float, [c_vp, c_int]),
     "logits_process": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_ll,
                                ctypes.POINTER(LogitsRules), c_vp]),
+    "rms_norm_forward": (c_int, [ctypes.POINTER(RmsNorm), c_vp]),
+    "rms_norm_backward": (c_int, [ctypes.POINTER(RmsNormGrad), c_vp]),
+    "rms_norm_backward_workspace": (c_size_t, [ctypes.POINTER(RmsNormGrad)]),
+    "quantize_rows": (c_int, [c_vp, c_ll, c_vp, c_vp, c_ll, c_int, c_int, c_int, c_vp]),
+    "rotary_frequencies": (c_int, [ctypes.POINTER(Rotary), c_double, c_int, c_double, c_int,
+                                   c_double, c_double]),
+    "rotary_forward": (c_int, [ctypes.POINTER(Rotary), c_vp, c_ll, c_vp, c_ll, c_int, c_int,
+                               c_int, c_vp, c_vp]),
+    "rotary_backward": (c_int, [ctypes.POINTER(Rotary), c_vp, c_ll, c_vp, c_ll, c_int, c_int,
+                                c_int, c_vp, c_vp]),
     # gpt.h
     "param_sizes": (None, [ctypes.POINTER(c_size_t), ctypes.POINTER(GPTConfig)]),
     "gpt_alloc": (None, [_GPTP]),
@@ -307,6 +355,18 @@ def batched_gemm(ta, tb, batch, M, N, K, alpha, A, sA, B, sB, beta, C, sC,
                        beta, C, sC, stream or None)
 
 
+# 8-bit linear layers. A call that the library refuses raises; the library's
+# message, on stderr, says why (here and below, for every call that returns a
+# status).
+def gemm_i8(g: GemmI8, stream=0) -> None:
+    if (_lib or lib()).gemm_i8(g, stream or None):
+        raise ValueError("gemm_i8 refused its arguments")
+
+
+def gemm_i8_workspace(g: GemmI8) -> int:
+    return lib().gemm_i8_workspace(g)
+
+
 # ------------------------------------------------------------ flash.h
 def flash_forward(out, lse, qkv, B, T, C, NH) -> None:
     lib().flash_attention_forward(out, lse, qkv, B, T, C, NH)
@@ -343,8 +403,7 @@ def flash_default_bwd_config() -> int:
     return int(lib().flash_default_bwd_config())
 
 
-# Generation (the paged key-value cache). A call that the library refuses
-# raises; the library's message, on stderr, says why.
+# Generation (the paged key-value cache).
 def paged_plan(plan: PagedPlan, stream=0) -> None:
     if (_lib or lib()).paged_plan(plan, stream or None):
         raise ValueError("paged_plan refused its arguments")
@@ -368,6 +427,46 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, out, lse, q, stream=0)
 def logits_process(out, logits, type, rows, V, stride, rules: LogitsRules, stream=0) -> None:
     if (_lib or lib()).logits_process(out, logits, type, rows, V, stride, rules, stream or None):
         raise ValueError("logits_process refused its arguments")
+
+
+def rms_norm_forward(norm: RmsNorm, stream=0) -> None:
+    if (_lib or lib()).rms_norm_forward(norm, stream or None):
+        raise ValueError("rms_norm_forward refused its arguments")
+
+
+def rms_norm_backward(grad: RmsNormGrad, stream=0) -> None:
+    if (_lib or lib()).rms_norm_backward(grad, stream or None):
+        raise ValueError("rms_norm_backward refused its arguments")
+
+
+def rms_norm_backward_workspace(grad: RmsNormGrad) -> int:
+    return lib().rms_norm_backward_workspace(grad)
+
+
+def quantize_rows(out, out_stride, scales, x, x_stride, type, rows, C, stream=0) -> None:
+    if (_lib or lib()).quantize_rows(out, out_stride, scales, x, x_stride, type, rows, C,
+                                     stream or None):
+        raise ValueError("quantize_rows refused its arguments")
+
+
+def rotary_frequencies(plan: Rotary, base, scaling=ROTARY_UNSCALED, factor=1.0, trained_len=0,
+                       slow=0.0, fast=0.0) -> None:
+    if lib().rotary_frequencies(plan, base, scaling, factor, trained_len, slow, fast):
+        raise ValueError("rotary_frequencies refused its arguments")
+
+
+def rotary_forward(plan: Rotary, out, out_stride, inp, inp_stride, type, tokens, heads, positions,
+                   stream=0) -> None:
+    if (_lib or lib()).rotary_forward(plan, out, out_stride, inp, inp_stride, type, tokens, heads,
+                                      positions, stream or None):
+        raise ValueError("rotary_forward refused its arguments")
+
+
+def rotary_backward(plan: Rotary, dinp, dinp_stride, dout, dout_stride, type, tokens, heads,
+                    positions, stream=0) -> None:
+    if (_lib or lib()).rotary_backward(plan, dinp, dinp_stride, dout, dout_stride, type, tokens,
+                                       heads, positions, stream or None):
+        raise ValueError("rotary_backward refused its arguments")
 
 
 def call(name, *args):

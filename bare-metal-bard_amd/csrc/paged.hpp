@@ -1,27 +1,17 @@
 // Shared pieces of the paged key-value cache kernels (paged.hip,
-// paged_attention.hip): element types, exact division by a page size, wave
-// scans, argument refusals.
+// paged_attention.hip): exact division by a page size, wave scans, the cache's
+// refusals.
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <stdint.h>
-#include <stdio.h>
 
 #include "../../include/flash.h"
+#include "args.hpp"
 #include "common.hpp"
 
 namespace bmb {
-
-// Prints why an entry point refuses its arguments; the caller returns -1.
-inline int refuse(const char *entry, const char *why) {
-    fprintf(stderr, "bmb: %s: %s\n", entry, why);
-    return -1;
-}
-
-inline int element_size(int type) {
-    return type == BMB_F32 ? 4 : type == BMB_F16 || type == BMB_BF16 ? 2 : 0;
-}
 
 // n / d and n % d for 0 <= n < 2^31 by one 64-bit product: with
 // s = ceil(log2 d) and m = ceil(2^(31+s) / d), m d exceeds 2^(31+s) by e < d

@@ -95,6 +95,37 @@ int gemm_set_math(int math);
 /* The mode gemm_set_math() last set (GEMM_MATH_BF16X3 before any call). */
 int gemm_get_math(void);
 
+/* No counterpart in the reference. A linear layer on 8-bit whole numbers, with
+ * a scale for each token (row of A) and each channel (row of B), as
+ * rms_norm_forward and quantize_rows (nn.h) make them:
+ *     C[m,n] = (sum_k A[m,k] * B[n,k]) * a_scales[m] * b_scales[n] + bias[n]
+ * The sum is exact (whole numbers in 32 bits, so K is at most 131071). It is
+ * rounded to fp32, so is its product with a_scales[m], and so is that product's
+ * with b_scales[n] together with the bias; the result is rounded to `type`. A, B and their strides are multiples of 16
+ * bytes; K is any number: what a row holds behind it has no influence, but up
+ * to the next multiple of 16 it is read. C needs its element's alignment;
+ * what lies between its rows is left as it was. C overlaps nothing else. */
+typedef struct GemmI8 {
+    int M, N, K;
+    int type; /* of C: BMB_F32 0, BMB_F16 1 or BMB_BF16 2 (nn.h) */
+    const signed char *A, *B;         /* (M, K), (N, K) */
+    const float *a_scales, *b_scales; /* (M), (N) */
+    const float *bias;                /* (N), or null */
+    void *C;                          /* (M, N) */
+    long long lda, ldb, ldc;          /* elements from row to row; lda and ldb below 2^23 */
+    void *work;                       /* device memory, used by one call at a time */
+    size_t work_bytes;
+} GemmI8;
+/* Queued on `stream` of the current device; returns 0, or -1 with a message on
+ * stderr, and nothing launched, for arguments it refuses. work: at least
+ * gemm_i8_workspace() bytes for the partial sums of a product that is split
+ * over K, which need no value; null: the call leases from the library's pool,
+ * as gemm() does, and does not split under graph capture. */
+int gemm_i8(const GemmI8 *g, hipStream_t stream BMB_DEFAULT_STREAM);
+/* Bytes of workspace for a call of these sizes (its pointers are not looked
+ * at); 0 if it needs none, or for sizes it would refuse. */
+size_t gemm_i8_workspace(const GemmI8 *g);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

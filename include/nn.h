@@ -28,12 +28,16 @@
 
 struct ihipStream_t; /* hipStream_t is a pointer to it */
 
-/* Element types of logits_process and of the paged cache (flash.h). */
+/* Element types of the operators below that take one, and of the paged cache
+ * (flash.h). */
 #ifndef BMB_F32
 #define BMB_F32 0
 #define BMB_F16 1
 #define BMB_BF16 2
 #endif
+/* 8-bit whole numbers with a scale for each row: a result of rms_norm_forward
+ * and quantize_rows, what gemm_i8 (gemm.h) multiplies. */
+#define BMB_I8 3
 
 #ifdef __cplusplus
 extern "C" {
@@ -143,6 +147,104 @@ typedef struct LogitsRules {
  * launched, for arguments it refuses. Allocates nothing. */
 int logits_process(void *out, const void *logits, int type, int rows, int V, long long stride,
                    const LogitsRules *rules, struct ihipStream_t *stream);
+
+/* ---- around the paged cache: a layer's norm, 8-bit rows, positions ----
+ * No counterpart in the reference. These calls are queued on `stream` of the
+ * current device, where all buffers live, and return 0, or -1 with a message
+ * on stderr, and nothing launched, for arguments they refuse. The structs are
+ * host memory, read during the call. Strides are elements from row to row, at
+ * least the row's width (0 for an input: one row for all); buffers need their
+ * element's alignment only, 16 bytes are fastest. Results overlap neither
+ * inputs nor each other unless said so; what lies between rows is left as it
+ * was. No result depends on anything but the inputs (no atomics). Nothing is
+ * allocated, so every call can be captured into a graph (rms_norm_backward
+ * with a workspace of the caller's).
+ *
+ * 8-bit rows: with a = the largest magnitude of the row's exact values v, q =
+ * 127 v / a rounded to the nearest whole number (the even one of two as near)
+ * and scale = a / 127, so that q * scale stands for v. A row of zeros has scale 0;
+ * one with an infinity or a NaN has q = 0 and scale NaN. q is never -128. */
+typedef struct RmsNorm {
+    int rows, C;  /* C up to 2^24 */
+    int type;     /* of x, residual and sum: BMB_F32, BMB_F16 or BMB_BF16 */
+    int out_type; /* of out: `type`, or BMB_I8 */
+    float eps;    /* > 0 */
+    const void *x, *residual; /* (rows, C); residual may be null */
+    void *sum;           /* x + residual, or null: not kept; may be x or residual */
+    const float *weight; /* (C) */
+    void *out;           /* (rows, C); of `type`, it may be x or residual */
+    float *scales;       /* (rows), with BMB_I8 */
+    float *rstd;         /* (rows) for the backward, or null */
+    long long x_stride, residual_stride, sum_stride, out_stride;
+} RmsNorm;
+/* s = x + residual, rounded to `type` (kept or not); rstd = 1 / sqrt(mean(s^2)
+ * + eps), the mean in 64 bits; out = s * rstd * weight. In 8 bits the row's
+ * values are the exact products s * weight, and rstd goes into the scale. */
+int rms_norm_forward(const RmsNorm *norm, struct ihipStream_t *stream);
+
+typedef struct RmsNormGrad {
+    int rows, C, type;   /* type: of dinp, dout, inp and dres; C up to 2^24 */
+    const void *dout;    /* gradient of out */
+    const void *inp;     /* what was normed: sum, or x where nothing was added */
+    const void *dres;    /* gradient that reaches the sum past the norm, or null */
+    const float *weight; /* (C) */
+    const float *rstd;   /* (rows), of the forward */
+    void *dinp;          /* gradient of x and of residual; may be dout, inp or dres */
+    float *dweight;      /* (C), or null */
+    long long dout_stride, inp_stride, dres_stride, dinp_stride;
+    void *work;          /* device memory, used by one call at a time */
+    size_t work_bytes;
+} RmsNormGrad;
+/* dinp = dres + rstd * (dout * weight - xhat * mean(dout * weight * xhat)) with
+ * xhat = inp * rstd; dweight += sum_rows dout * xhat. The sums over rows are
+ * fp32 over at most 64 rows at a time and 64 bits over those. work: at least
+ * rms_norm_backward_workspace() bytes, which need no value; null: the call
+ * leases from the library's pool, and is refused under graph capture if it
+ * needs any. */
+int rms_norm_backward(const RmsNormGrad *grad, struct ihipStream_t *stream);
+/* Bytes of workspace for a call of these sizes (its pointers but for dweight
+ * are not looked at); 0 if it needs none, or for sizes it would refuse. */
+size_t rms_norm_backward_workspace(const RmsNormGrad *grad);
+
+/* out, scales = the rows of x in 8 bits: activations that follow no norm (one
+ * scale a token), or weights (out_features, in_features) (one a channel).
+ * `type`: BMB_F32, BMB_F16 or BMB_BF16; C up to 2^24. */
+int quantize_rows(signed char *out, long long out_stride, float *scales, const void *x,
+                  long long x_stride, int type, int rows, int C, struct ihipStream_t *stream);
+
+/* Rotary positions. Pair i of the first `dims` of a head's elements turns by
+ * position * freq[i] radians and is multiplied by `amplitude`; the others pass
+ * unchanged. */
+#define BMB_ROTARY_HALF 0  /* pair i: elements i and i + dims / 2 */
+#define BMB_ROTARY_PAIRS 1 /* pair i: elements 2i and 2i + 1 */
+typedef struct Rotary {
+    int head_size, dims; /* head_size up to 256; dims even, 2 to head_size */
+    int layout;
+    float amplitude;     /* 1 as a rule */
+    double freq[128];    /* dims / 2 of them, from rotary_frequencies or the caller's */
+} Rotary;
+/* Frequencies base^(-2i / dims), for contexts `factor` times as long as those
+ * trained on: */
+#define BMB_ROTARY_UNSCALED 0 /* as they are */
+#define BMB_ROTARY_LINEAR 1   /* / factor */
+#define BMB_ROTARY_BASE 2     /* of base * factor^(dims / (dims - 2)) (dims 2: as they are) */
+#define BMB_ROTARY_PARTS 3    /* those that turn slow times or less over trained_len positions: / factor; */
+                              /* fast times or more: as they are; between: evenly from one to the other */
+/* Fills plan->freq on the host; launches nothing. factor >= 1; trained_len,
+ * slow and fast (0 <= slow < fast) are looked at for BMB_ROTARY_PARTS only. */
+int rotary_frequencies(Rotary *plan, double base, int scaling, double factor, int trained_len,
+                       double slow, double fast);
+/* Turns the first `heads` heads (heads * head_size elements) of each of
+ * `tokens` rows of `type`: queries and keys of fused QKV rows in one call.
+ * positions: (tokens), any number. out may be inp (with its stride). The angle
+ * is formed in 64 bits and reduced there. */
+int rotary_forward(const Rotary *plan, void *out, long long out_stride, const void *inp,
+                   long long inp_stride, int type, int tokens, int heads, const int *positions,
+                   struct ihipStream_t *stream);
+/* dinp = what the forward's transpose makes of dout; dinp may be dout. */
+int rotary_backward(const Rotary *plan, void *dinp, long long dinp_stride, const void *dout,
+                    long long dout_stride, int type, int tokens, int heads, const int *positions,
+                    struct ihipStream_t *stream);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus
