@@ -4,8 +4,6 @@
 // l supplies 16 consecutive bytes of row l % 32 at k = 16 (l / 32), and since
 // both supply the same k in the same place, their order inside the instruction
 // does not matter. Sums are whole numbers in 32 bits: exact, in any order.
-// B goes in as the instruction's first operand, so a lane holds four
-// consecutive columns of C in four registers.
 //
 // A stage is 128 k. Its tile of A and of B goes from global memory straight
 // into LDS (16 bytes a lane, no registers), rows of 128 bytes whose eight
@@ -54,31 +52,31 @@ struct I8Tile {
 typedef __attribute__((address_space(3))) void lds_void;
 
 // ROWS rows of one operand's stage into LDS: lane i of a wave fills the i-th
-// chunk of 1 KB, eight rows.
+// chunk of 1 KB, eight rows; the workgroup's load i rows i * STEP on, where a
+// chunk's place in its row is the same (STEP is a multiple of 16).
 template <int ROWS, int NT>
 struct Staging {
-    static constexpr int LOADS = ROWS * CHUNKS / NT;
-    int row[LOADS];  // byte offset of this lane's row
-    int chunk[LOADS];
+    static constexpr int LOADS = ROWS * CHUNKS / NT, STEP = NT / CHUNKS;
+    static_assert(STEP % 16 == 0, "chunks move with their row modulo 16");
+    int row, chunk;       // byte offsets of this lane's first row, and in it
+    int step, last_row;  // of the next load's row, and of the operand's last row
     __device__ __forceinline__ void setup(int rows, int ld) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int at = i * NT + threadIdx.x, r = at / CHUNKS;
-            row[i] = min(r, rows - 1) * ld;
-            chunk[i] = ((at % CHUNKS) ^ ((r >> 1) & 7)) * CHUNK;
-        }
+        const int r = threadIdx.x / CHUNKS;
+        row = r * ld;
+        chunk = ((threadIdx.x % CHUNKS) ^ ((r >> 1) & 7)) * CHUNK;
+        step = STEP * ld;
+        last_row = (min(rows, ROWS) - 1) * ld;
     }
-    // k0: the stage's first k; last: the first k of the operand's last chunk.
-    template <bool WHOLE>
-    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t p, char *lds, int k0,
-                                         int last) const {
+    // Load i of a stage. k0: the stage's first k; last: the first k of the
+    // operand's last chunk.
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t p, char *lds, int k0, int last,
+                                         int i) const {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            char *to = lds + (i * NT + wave * 64) * CHUNK;
-            const int off = WHOLE ? row[i] + chunk[i] : row[i] + min(chunk[i], last - k0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(p, (lds_void *)to, 16, off, k0, 0, 0);
-        }
+        [[maybe_unused]] char *to = lds + (i * NT + wave * 64) * CHUNK;
+        [[maybe_unused]] const int at = min(row + i * step, last_row) + min(chunk + k0, last);
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass does not know loads of 16 bytes)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(p, (lds_void *)to, 16, at, 0, 0, 0);
+#endif
     }
 };
 
@@ -87,9 +85,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const signed char *p) 
                                              0x00027000);
 }
 
-// Chunk c of row r of a staged tile.
-__device__ __forceinline__ i32x4 chunk_at(const char *lds, int r, int c) {
-    return *(const i32x4 *)(lds + r * BK + ((c ^ ((r >> 1) & 7)) * CHUNK));
+// Where this lane finds its operand of a stage's first step in row r of the
+// tile; those of step kk are at place ^ 32 kk, and of rows 32 i on 4096 i on.
+__device__ __forceinline__ int place_of(int r, int half) {
+    return r * BK + ((half ^ ((r >> 1) & 7)) * CHUNK);
+}
+__device__ __forceinline__ i32x4 operand_at(const char *lds, int place, int kk, int i) {
+    return *(const i32x4 *)(lds + ((place ^ (32 * kk)) + i * 32 * BK));
 }
 
 // The first n bytes of a chunk (n any number).
@@ -102,6 +104,12 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 x, int n) {
     return x;
 }
 
+// A wave's operands of one step of 32 k.
+template <int FM, int FN>
+struct Operands {
+    i32x4 a[FM], b[FN];
+};
+
 template <typename Tile, typename T>
 __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN;
@@ -109,6 +117,9 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     // loads into the other.
     __shared__ __attribute__((aligned(256))) char a0[BM * BK], a1[BM * BK];
     __shared__ __attribute__((aligned(256))) char b0[BN * BK], b1[BN * BK];
+    // Read back with the results: loads from memory there would wait for the stores
+    // before them.
+    __shared__ float scale_m[BM], scale_n[BN], bias_n[BN];
     int tm, tn;
     group_tile(xcd_remap((int)blockIdx.x, (int)gridDim.x), a.tiles_m, a.tiles_n, 8, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
@@ -118,76 +129,154 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     Staging<BN, Tile::NT> sb;
     sa.setup(a.M - m0, (int)a.lda);
     sb.setup(a.N - n0, (int)a.ldb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < BM; i += Tile::NT) scale_m[i] = a.a_scales[min(m0 + i, a.M - 1)];
+    for (int i = threadIdx.x; i < BN; i += Tile::NT) {
+        scale_n[i] = a.b_scales[min(n0 + i, a.N - 1)];
+        bias_n[i] = a.bias ? a.bias[min(n0 + i, a.N - 1)] : 0.0f;
+    }
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / Tile::WAVES_N * Tile::WM, wn = wave % Tile::WAVES_N * Tile::WN;
     const int r = lane & 31, half = lane >> 5;
 
+    int place_a = place_of(wm + r, half), place_b = place_of(wn + r, half);
+
     i32x16 acc[FM][FN] = {};
-    const auto load = [&](char *la, char *lb, int k0) {
-        if (k0 + BK <= a.K) {
-            sa.template load<true>(A, la, k0, 0);
-            sb.template load<true>(B, lb, k0, 0);
-        } else if (k0 < a.K) {
-            const int last = (a.K - 1) / CHUNK * CHUNK;
-            sa.template load<false>(A, la, k0, last);
-            sb.template load<false>(B, lb, k0, last);
+    // Operands of one step of 32 k, and of the next while it is multiplied.
+    typedef Operands<FM, FN> Step;
+    Step even, odd;
+    const int last = (a.K - 1) / CHUNK * CHUNK;
+    constexpr int LOADS = decltype(sa)::LOADS + decltype(sb)::LOADS;
+    const auto load = [&](char *la, char *lb, int k0, int i) {
+        if (i < decltype(sa)::LOADS)
+            sa.load(A, la, k0, last, i);
+        else
+            sb.load(B, lb, k0, last, i - decltype(sa)::LOADS);
+    };
+    // Read i of a step's operands, in the order in which the products want them.
+    const auto read = [&](Step &f, const char *la, const char *lb, int kk, int i) {
+        if (i == 0 || i > FN)
+            f.a[i ? i - FN : 0] = operand_at(la, place_a, kk, i ? i - FN : 0);
+        else
+            f.b[i - 1] = operand_at(lb, place_b, kk, i - 1);
+    };
+    const auto product = [&](const Step &f, int t) {
+        const int i = t / FN, j = t % FN;
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+    };
+    // One step: its products, and between them the reads of the next step's
+    // operands (step kk of stage la, lb) and loads [first, first + n) of stage
+    // k0 into ga, gb, if there is `more`. Fenced, since the compiler gathers them.
+    const auto step = [&](const Step &now, Step &next, const char *la, const char *lb, int kk,
+                          char *ga, char *gb, int k0, int first, int n, bool more) {
+        // (not all steps' places at once: they do not fit the registers)
+        asm volatile("" : "+v"(place_a), "+v"(place_b));
+#pragma unroll
+        for (int t = 0; t < FM * FN; ++t) {
+#pragma unroll
+            for (int i = t * (FM + FN) / (FM * FN); i < (t + 1) * (FM + FN) / (FM * FN); ++i)
+                read(next, la, lb, kk, i);
+#pragma unroll
+            for (int i = t * n / (FM * FN); i < (t + 1) * n / (FM * FN); ++i)
+                if (more) load(ga, gb, k0, first + i);
+            product(now, t);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    const auto multiply = [&](const char *la, const char *lb, int k0) {
-        const bool whole = k0 + BK <= a.K;
+    // Stage k0 (the operands of its first step are read, the next stage's last
+    // loads not yet issued) up to the first step of the next. The loads are
+    // spread over three steps: a wave that issues them all at once waits until
+    // the memory pipeline has taken them.
+    constexpr int L0 = (3 * LOADS + 7) / 8, L1 = L0, L2 = LOADS - L0 - L1;
+    const auto stage = [&](char *la, char *lb, char *na, char *nb, int k0, bool more) {
+        step(even, odd, la, lb, 1, na, nb, k0 + BK, L0, L1, true);
+        step(odd, even, la, lb, 2, na, nb, k0 + BK, L0 + L1, L2, true);
+        step(even, odd, la, lb, 3, na, nb, 0, 0, 0, true);
+        // This wave has read the stage, and its loads of the next are in LDS; behind
+        // the barrier everybody's are.
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+        __syncthreads();
+        step(odd, even, na, nb, 0, la, lb, k0 + 2 * BK, 0, L0, more);
+    };
+    // The last stage.
+    const auto finish = [&](const char *la, const char *lb, int k0) {
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
-            i32x4 fa[FM], fb[FN];
+            if (kk > 0) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = chunk_at(la, wm + i * 32 + r, 2 * kk + half);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = chunk_at(lb, wn + j * 32 + r, 2 * kk + half);
-            if (!whole) {
+                for (int i = 0; i < FM + FN; ++i) read(even, la, lb, kk, i);
+            }
+            if (k0 + BK > a.K) {
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
-                    fa[i] = first_bytes(fa[i], a.K - k0 - (2 * kk + half) * CHUNK);
+                    even.a[i] = first_bytes(even.a[i], a.K - k0 - (2 * kk + half) * CHUNK);
             }
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+            for (int t = 0; t < FM * FN; ++t) product(even, t);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    if (a.K > 0) {
 #pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < LOADS; ++i) load(a0, b0, 0, i);
+        if (a.K > BK) {
+#pragma unroll
+            for (int i = 0; i < L0; ++i) load(a1, b1, BK, i);
+            __builtin_amdgcn_s_waitcnt(0x0f70 | L0);
+        } else {
+            __builtin_amdgcn_s_waitcnt(0x0f70);
         }
-    };
-    // vmcnt(0): this wave's loads are in LDS; the barrier: everybody's are.
-    const auto ready = [] {
-        __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();
-    };
-    load(a0, b0, 0);
-    for (int k0 = 0; k0 < a.K; k0 += 2 * BK) {
-        ready();
-        load(a1, b1, k0 + BK);
-        multiply(a0, b0, k0);
-        ready();
-        if (k0 + BK < a.K) {
-            load(a0, b0, k0 + 2 * BK);
-            multiply(a1, b1, k0 + BK);
+#pragma unroll
+        for (int i = 0; i < FM + FN; ++i) read(even, a0, b0, 0, i);
+        int k0 = 0;
+        const char *la = a0, *lb = b0;
+        for (; k0 + 2 * BK < a.K; k0 += 2 * BK) {
+            stage(a0, b0, a1, b1, k0, true);
+            stage(a1, b1, a0, b0, k0 + BK, k0 + 3 * BK < a.K);
         }
+        if (k0 + BK < a.K) {
+            stage(a0, b0, a1, b1, k0, false);
+            k0 += BK;
+            la = a1;
+            lb = b1;
+        }
+        finish(la, lb, k0);
     }
 
-    // Lane: row l % 32 of C, columns 8 g + 4 (l / 32) + 0..3 in registers 4 g + 0..3.
+    // Lane: column l % 32 of C, rows 8 g + 4 (l / 32) + 0..3 in registers 4 g + 0..3:
+    // a store fills 32 columns of two rows. Rows are uniform but for half.
+    const unsigned sub = 4u * half * (unsigned)a.ldc + r;
+    const bool inside = m0 + BM <= a.M && n0 + BN <= a.N;
+    __syncthreads();  // (K = 0: the scales are in LDS)
+    float sn[FN], bias[FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int m = m0 + wm + i * 32 + r;
-        if (m >= a.M) continue;
-        const float sm = a.a_scales[m];
-        T *row = (T *)a.C + m * a.ldc;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int n = n0 + wn + j * 32 + 8 * (e / 4) + 4 * half + e % 4;
-                if (n >= a.N) continue;
-                const float y = (float)acc[i][j][e] * sm;
-                row[n] = (T)__builtin_fmaf(y, a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
-            }
+    for (int j = 0; j < FN; ++j) {
+        sn[j] = scale_n[wn + j * 32 + r];
+        bias[j] = bias_n[wn + j * 32 + r];
     }
+    T *row = (T *)a.C + (m0 + wm) * a.ldc + (n0 + wn);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 sm = *(const float4 *)(scale_m + wm + i * 32 + 8 * g + 4 * half);
+            const float each[4] = {sm.x, sm.y, sm.z, sm.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int m = m0 + wm + i * 32 + 8 * g + e + 4 * half;
+                if (inside || m < a.M) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+                        if (inside || n0 + wn + j * 32 + r < a.N)
+                            row[sub + j * 32] = (T)__builtin_fmaf(
+                                (float)acc[i][j][4 * g + e] * each[e], sn[j], bias[j]);
+                }
+                row += e == 3 ? 5 * a.ldc : a.ldc;
+                // (one row after the other: all rows' addresses at once do not fit the registers)
+                asm volatile("" : "+s"(row));
+            }
+        }
 }
 
 template <typename Tile, typename T>
