@@ -31,7 +31,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int MAX_K = 131071;      // 128 * 128 * MAX_K < 2^31
-constexpr int BK = 128, CHUNK = 16, CHUNKS = BK / CHUNK;
+constexpr int CHUNK = 16;
 
 struct I8Args {
     const signed char *A, *B;
@@ -42,28 +42,45 @@ struct I8Args {
     long long first;
 };
 
-template <int BM_, int BN_, int WAVES_M_, int WAVES_N_>
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int BK_>
 struct I8Tile {
-    static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
+    static constexpr int BM = BM_, BN = BN_, BK = BK_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
     static constexpr int NT = 64 * WAVES_M * WAVES_N;
     static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 32, FN = WN / 32;
 };
 
 typedef __attribute__((address_space(3))) void lds_void;
 
+// A stage's rows in LDS: BK bytes, their 16-byte chunks permuted by the row so
+// that the groups of 16 lanes in which a 128-bit read of 32 rows is served, {0-3,
+// 12-15, 20-27}, {4-11, 16-19, 28-31}, touch 16 different places modulo 256
+// bytes. Rows of 64 bytes also swap places in pairs.
+template <int BK>
+struct Layout {
+    static constexpr int CHUNKS = BK / CHUNK;
+    static_assert(BK == 64 || BK == 128, "the permutations are these two's");
+    __device__ static __forceinline__ int slot(int row) {  // of a row (and row of a slot)
+        return BK == 64 ? row ^ ((row >> 2) & 1) : row;
+    }
+    __device__ static __forceinline__ int permuted(int row, int chunk) {
+        return chunk ^ (BK == 64 ? (row >> 3) & 3 : (row >> 1) & 7);
+    }
+};
+
 // ROWS rows of one operand's stage into LDS: lane i of a wave fills the i-th
-// chunk of 1 KB, eight rows; the workgroup's load i rows i * STEP on, where a
-// chunk's place in its row is the same (STEP is a multiple of 16).
-template <int ROWS, int NT>
+// chunk of 1 KB; the workgroup's load i rows i * STEP on, where rows and chunks
+// are permuted alike (STEP is a multiple of 32).
+template <int ROWS, int NT, int BK>
 struct Staging {
-    static constexpr int LOADS = ROWS * CHUNKS / NT, STEP = NT / CHUNKS;
-    static_assert(STEP % 16 == 0, "chunks move with their row modulo 16");
-    int row, chunk;       // byte offsets of this lane's first row, and in it
+    typedef Layout<BK> L;
+    static constexpr int LOADS = ROWS * L::CHUNKS / NT, STEP = NT / L::CHUNKS;
+    static_assert(STEP % 32 == 0, "permutations depend on the row modulo 32");
+    int row, chunk;      // byte offsets of this lane's first row, and in it
     int step, last_row;  // of the next load's row, and of the operand's last row
     __device__ __forceinline__ void setup(int rows, int ld) {
-        const int r = threadIdx.x / CHUNKS;
+        const int slot = threadIdx.x / L::CHUNKS, r = L::slot(slot);
         row = r * ld;
-        chunk = ((threadIdx.x % CHUNKS) ^ ((r >> 1) & 7)) * CHUNK;
+        chunk = L::permuted(r, threadIdx.x % L::CHUNKS) * CHUNK;
         step = STEP * ld;
         last_row = (min(rows, ROWS) - 1) * ld;
     }
@@ -86,10 +103,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const signed char *p) 
 }
 
 // Where this lane finds its operand of a stage's first step in row r of the
-// tile; those of step kk are at place ^ 32 kk, and of rows 32 i on 4096 i on.
+// tile; those of step kk are at place ^ 32 kk, and of rows 32 i on 32 i rows on.
+template <int BK>
 __device__ __forceinline__ int place_of(int r, int half) {
-    return r * BK + ((half ^ ((r >> 1) & 7)) * CHUNK);
+    return Layout<BK>::slot(r) * BK + Layout<BK>::permuted(r, half) * CHUNK;
 }
+template <int BK>
 __device__ __forceinline__ i32x4 operand_at(const char *lds, int place, int kk, int i) {
     return *(const i32x4 *)(lds + ((place ^ (32 * kk)) + i * 32 * BK));
 }
@@ -104,6 +123,15 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 x, int n) {
     return x;
 }
 
+// A barrier that waits for nothing but the other waves (__syncthreads() also
+// waits for every load into LDS that is on its way). The caller has waited for
+// what the others will read.
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // A wave's operands of one step of 32 k.
 template <int FM, int FN>
 struct Operands {
@@ -112,63 +140,62 @@ struct Operands {
 
 template <typename Tile, typename T>
 __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
-    constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN;
+    constexpr int BM = Tile::BM, BN = Tile::BN, BK = Tile::BK, FM = Tile::FM, FN = Tile::FN;
     // Objects of their own, so that reads of one stage do not wait for the
     // loads into the other.
-    __shared__ __attribute__((aligned(256))) char a0[BM * BK], a1[BM * BK];
+    __shared__ __attribute__((aligned(256))) char a0[BM * BK], a1[BM * BK], a2[BM * BK];
     __shared__ __attribute__((aligned(256))) char b0[BN * BK], b1[BN * BK];
-    // Read back with the results: loads from memory there would wait for the stores
-    // before them.
-    __shared__ float scale_m[BM], scale_n[BN], bias_n[BN];
     int tm, tn;
     group_tile(xcd_remap((int)blockIdx.x, (int)gridDim.x), a.tiles_m, a.tiles_n, 8, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const __amdgpu_buffer_rsrc_t A = operand(a.A + (long long)m0 * a.lda);
     const __amdgpu_buffer_rsrc_t B = operand(a.B + (long long)n0 * a.ldb);
-    Staging<BM, Tile::NT> sa;
-    Staging<BN, Tile::NT> sb;
+    Staging<BM, Tile::NT, BK> sa;
+    Staging<BN, Tile::NT, BK> sb;
     sa.setup(a.M - m0, (int)a.lda);
     sb.setup(a.N - n0, (int)a.ldb);
-    for (int i = threadIdx.x; i < BM; i += Tile::NT) scale_m[i] = a.a_scales[min(m0 + i, a.M - 1)];
-    for (int i = threadIdx.x; i < BN; i += Tile::NT) {
-        scale_n[i] = a.b_scales[min(n0 + i, a.N - 1)];
-        bias_n[i] = a.bias ? a.bias[min(n0 + i, a.N - 1)] : 0.0f;
-    }
+    static_assert(BM <= Tile::NT && BN <= Tile::NT, "a scale a thread");
+    const int tid = threadIdx.x;
+    const float scale_of_m = a.a_scales[min(m0 + min(tid, BM - 1), a.M - 1)];
+    const float scale_of_n = a.b_scales[min(n0 + min(tid, BN - 1), a.N - 1)];
+    const float bias_of_n = a.bias ? a.bias[min(n0 + min(tid, BN - 1), a.N - 1)] : 0.0f;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / Tile::WAVES_N * Tile::WM, wn = wave % Tile::WAVES_N * Tile::WN;
     const int r = lane & 31, half = lane >> 5;
 
-    int place_a = place_of(wm + r, half), place_b = place_of(wn + r, half);
+    int place_a = place_of<BK>(wm + r, half), place_b = place_of<BK>(wn + r, half);
 
     i32x16 acc[FM][FN] = {};
     // Operands of one step of 32 k, and of the next while it is multiplied.
     typedef Operands<FM, FN> Step;
     Step even, odd;
     const int last = (a.K - 1) / CHUNK * CHUNK;
-    constexpr int LOADS = decltype(sa)::LOADS + decltype(sb)::LOADS;
-    const auto load = [&](char *la, char *lb, int k0, int i) {
-        if (i < decltype(sa)::LOADS)
-            sa.load(A, la, k0, last, i);
-        else
-            sb.load(B, lb, k0, last, i - decltype(sa)::LOADS);
+    constexpr int LA = decltype(sa)::LOADS, LB = decltype(sb)::LOADS;
+    // Load i of a pair of stages: of B's stage kb into lb, then of A's stage ka into la.
+    const auto load = [&](char *la, int ka, char *lb, int kb, int i) {
+        if (i < LB) {
+            if (kb < a.K) sb.load(B, lb, kb, last, i);
+        } else {
+            if (ka < a.K) sa.load(A, la, ka, last, i - LB);
+        }
     };
     // Read i of a step's operands, in the order in which the products want them.
     const auto read = [&](Step &f, const char *la, const char *lb, int kk, int i) {
         if (i == 0 || i > FN)
-            f.a[i ? i - FN : 0] = operand_at(la, place_a, kk, i ? i - FN : 0);
+            f.a[i ? i - FN : 0] = operand_at<BK>(la, place_a, kk, i ? i - FN : 0);
         else
-            f.b[i - 1] = operand_at(lb, place_b, kk, i - 1);
+            f.b[i - 1] = operand_at<BK>(lb, place_b, kk, i - 1);
     };
     const auto product = [&](const Step &f, int t) {
         const int i = t / FN, j = t % FN;
         acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
     };
     // One step: its products, and between them the reads of the next step's
-    // operands (step kk of stage la, lb) and loads [first, first + n) of stage
-    // k0 into ga, gb, if there is `more`. Fenced, since the compiler gathers them.
+    // operands (step kk of stage la, lb) and loads [first, first + n) of a pair of
+    // stages into ga, gb. Fenced, since the compiler gathers them.
     const auto step = [&](const Step &now, Step &next, const char *la, const char *lb, int kk,
-                          char *ga, char *gb, int k0, int first, int n, bool more) {
+                          char *ga, int ka, char *gb, int kb, int first, int n) {
         // (not all steps' places at once: they do not fit the registers)
         asm volatile("" : "+v"(place_a), "+v"(place_b));
 #pragma unroll
@@ -178,38 +205,46 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
                 read(next, la, lb, kk, i);
 #pragma unroll
             for (int i = t * n / (FM * FN); i < (t + 1) * n / (FM * FN); ++i)
-                if (more) load(ga, gb, k0, first + i);
+                load(ga, ka, gb, kb, first + i);
             product(now, t);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Stage k0 (the operands of its first step are read, the next stage's last
-    // loads not yet issued) up to the first step of the next. The loads are
-    // spread over three steps: a wave that issues them all at once waits until
-    // the memory pipeline has taken them.
-    constexpr int L0 = (3 * LOADS + 7) / 8, L1 = L0, L2 = LOADS - L0 - L1;
-    const auto stage = [&](char *la, char *lb, char *na, char *nb, int k0, bool more) {
-        step(even, odd, la, lb, 1, na, nb, k0 + BK, L0, L1, true);
-        step(odd, even, la, lb, 2, na, nb, k0 + BK, L0 + L1, L2, true);
-        step(even, odd, la, lb, 3, na, nb, 0, 0, 0, true);
-        // This wave has read the stage, and its loads of the next are in LDS; behind
-        // the barrier everybody's are.
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
-        __syncthreads();
-        step(odd, even, na, nb, 0, la, lb, k0 + 2 * BK, 0, L0, more);
+    // Stage k0 in la, lb (the operands of its first step are read) up to the first
+    // step of the next in na, nb. Behind the barrier its places are free for
+    // A's stage after the next two and B's after the next; these loads (the first
+    // L0 in the last step, the others in the next stage, whose `la` and `lb` before
+    // are pa, pb) are spread over the steps: a wave that issues them all at once
+    // waits until the memory pipeline has taken them.
+    constexpr int STEPS = BK / 32, LOADS = LA + LB, L0 = (3 * LOADS + 7) / 8;
+    constexpr int L1 = STEPS == 2 ? LOADS - L0 : L0, L2 = LOADS - L0 - L1;
+    const auto stage = [&](char *pa, char *pb, char *la, char *lb, const char *na, const char *nb,
+                           int k0) {
+        step(even, odd, la, lb, 1, pa, k0 + 2 * BK, pb, k0 + BK, L0, L1);
+        if constexpr (STEPS == 4) {
+            step(odd, even, la, lb, 2, pa, k0 + 2 * BK, pb, k0 + BK, L0 + L1, L2);
+            step(even, odd, la, lb, 3, pa, 0, pb, 0, 0, 0);
+        }
+        // This wave has read the stage, and its loads of the next are in LDS (A's of
+        // the one behind it may be on their way); behind the barrier everybody's are.
+        __builtin_amdgcn_s_waitcnt(0x0070 | LA);  // vmcnt(LA), lgkmcnt(0)
+        if (k0 + 2 * BK >= a.K) __builtin_amdgcn_s_waitcnt(0x0070);
+        barrier();
+        step(odd, even, na, nb, 0, la, k0 + 3 * BK, lb, k0 + 2 * BK, 0, L0);
     };
-    // The last stage.
-    const auto finish = [&](const char *la, const char *lb, int k0) {
+    // The last stage, of `rest` k.
+    int rest = 0;
+    const auto finish = [&](const char *la, const char *lb) {
 #pragma unroll
-        for (int kk = 0; kk < BK / 32; ++kk) {
+        for (int kk = 0; kk < STEPS; ++kk) {
             if (kk > 0) {
 #pragma unroll
                 for (int i = 0; i < FM + FN; ++i) read(even, la, lb, kk, i);
             }
-            if (k0 + BK > a.K) {
+            if (rest < BK) {
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
-                    even.a[i] = first_bytes(even.a[i], a.K - k0 - (2 * kk + half) * CHUNK);
+                    even.a[i] = first_bytes(even.a[i], rest - (2 * kk + half) * CHUNK);
             }
 #pragma unroll
             for (int t = 0; t < FM * FN; ++t) product(even, t);
@@ -218,37 +253,65 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     };
     if (a.K > 0) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) load(a0, b0, 0, i);
-        if (a.K > BK) {
+        for (int i = 0; i < LOADS; ++i) load(a0, 0, b0, 0, i);
 #pragma unroll
-            for (int i = 0; i < L0; ++i) load(a1, b1, BK, i);
-            __builtin_amdgcn_s_waitcnt(0x0f70 | L0);
-        } else {
-            __builtin_amdgcn_s_waitcnt(0x0f70);
-        }
-        __syncthreads();
+        for (int i = LB; i < LOADS; ++i) load(a1, BK, b1, BK, i);
+#pragma unroll
+        for (int i = 0; i < L0; ++i) load(a2, 2 * BK, b1, BK, i);
+        static_assert(L0 <= LB, "the loads behind the first two stages' A are B's");
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (LA + L0));
+        if (a.K <= 2 * BK) __builtin_amdgcn_s_waitcnt(0x0f70);
+        barrier();
 #pragma unroll
         for (int i = 0; i < FM + FN; ++i) read(even, a0, b0, 0, i);
         int k0 = 0;
+        for (; k0 + 6 * BK < a.K; k0 += 6 * BK) {
+            stage(a2, b1, a0, b0, a1, b1, k0);
+            stage(a0, b0, a1, b1, a2, b0, k0 + BK);
+            stage(a1, b1, a2, b0, a0, b1, k0 + 2 * BK);
+            stage(a2, b0, a0, b1, a1, b0, k0 + 3 * BK);
+            stage(a0, b1, a1, b0, a2, b1, k0 + 4 * BK);
+            stage(a1, b0, a2, b1, a0, b0, k0 + 5 * BK);
+        }
+        rest = a.K - k0;
         const char *la = a0, *lb = b0;
-        for (; k0 + 2 * BK < a.K; k0 += 2 * BK) {
-            stage(a0, b0, a1, b1, k0, true);
-            stage(a1, b1, a0, b0, k0 + BK, k0 + 3 * BK < a.K);
+        const auto left = [&](const char *na, const char *nb) {
+            rest -= BK;
+            la = na;
+            lb = nb;
+            return rest > BK;
+        };
+        if (rest > BK) {
+            stage(a2, b1, a0, b0, a1, b1, k0);
+            if (left(a1, b1)) {
+                stage(a0, b0, a1, b1, a2, b0, k0 + BK);
+                if (left(a2, b0)) {
+                    stage(a1, b1, a2, b0, a0, b1, k0 + 2 * BK);
+                    if (left(a0, b1)) {
+                        stage(a2, b0, a0, b1, a1, b0, k0 + 3 * BK);
+                        if (left(a1, b0)) {
+                            stage(a0, b1, a1, b0, a2, b1, k0 + 4 * BK);
+                            left(a2, b1);
+                        }
+                    }
+                }
+            }
         }
-        if (k0 + BK < a.K) {
-            stage(a0, b0, a1, b1, k0, false);
-            k0 += BK;
-            la = a1;
-            lb = b1;
-        }
-        finish(la, lb, k0);
+        finish(la, lb);
     }
 
     // Lane: column l % 32 of C, rows 8 g + 4 (l / 32) + 0..3 in registers 4 g + 0..3:
     // a store fills 32 columns of two rows. Rows are uniform but for half.
     const unsigned sub = 4u * half * (unsigned)a.ldc + r;
     const bool inside = m0 + BM <= a.M && n0 + BN <= a.N;
-    __syncthreads();  // (K = 0: the scales are in LDS)
+    // The scales by LDS, whose stages have been read: loads from memory there would
+    // wait for the stores before them.
+    float *scale_m = (float *)a0, *scale_n = scale_m + BM, *bias_n = scale_n + BN;
+    __syncthreads();
+    if (tid < BM) scale_m[tid] = scale_of_m;
+    if (tid < BN) scale_n[tid] = scale_of_n;
+    if (tid < BN) bias_n[tid] = bias_of_n;
+    __syncthreads();
     float sn[FN], bias[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -292,11 +355,11 @@ void launch_i8(I8Args &a, hipStream_t stream) {
         return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn);
     };
     if (tiles(256, 256) >= 256)
-        launch_tile<I8Tile<256, 256, 2, 4>, T>(a, stream);
+        launch_tile<I8Tile<256, 256, 2, 4, 128>, T>(a, stream);
     else if (tiles(128, 128) >= 256)
-        launch_tile<I8Tile<128, 128, 2, 2>, T>(a, stream);
+        launch_tile<I8Tile<128, 128, 2, 2, 128>, T>(a, stream);
     else
-        launch_tile<I8Tile<64, 64, 2, 2>, T>(a, stream);
+        launch_tile<I8Tile<64, 64, 2, 2, 128>, T>(a, stream);
 }
 
 const char *size_fault(const GemmI8 *g) {
