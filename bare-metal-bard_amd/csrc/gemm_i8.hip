@@ -5,12 +5,16 @@
 // both supply the same k in the same place, their order inside the instruction
 // does not matter. Sums are whole numbers in 32 bits: exact, in any order.
 //
-// A stage is 128 k. Its tile of A and of B goes from global memory straight
-// into LDS (16 bytes a lane, no registers), rows of 128 bytes whose eight
-// 16-byte chunks are permuted by their row (chunk ^ (row / 2) % 8): the groups of 16
-// lanes that a 128-bit read is served in then touch 16 different places
-// modulo 256 bytes. Two stages in turn; the loads of the next are on their way
-// while one is multiplied.
+// A stage is 128 k (64 where few k leave the results' bytes the bound). Its tile
+// of A and of B goes from global memory straight into LDS (16 bytes a lane, no
+// registers). LDS holds three stages of A and two of B (all 160 KB for 256 x 256
+// tiles): what bounds a tile is how long before its use a load is issued. In
+// steps of 32 k a wave multiplies what it has read, and between the products
+// reads the next step's operands and issues loads; one barrier a stage. 8192^3
+// (256 x 256 tiles): two stages of both, all loads at the stage's start 525 us;
+// spread 510; scales by LDS instead of from memory between the stores, which
+// waited for the stores, 477; A three stages deep 446 (2470 TOP/s; on zeros
+// 365: the matrix cores run at 1.7 of 2.4 GHz, held back by power).
 //
 // Edges. Rows past the last are loaded from the last one and reach only
 // results that are not stored. In a last stage that is not whole, chunks past
@@ -18,9 +22,13 @@
 // to zero before they are multiplied (so B's need no mask).
 #include <limits.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "args.hpp"
 #include "common.hpp"
 #include "launch.hpp"
+#include "paged.hpp"
 #include "workspace.hpp"
 #include "../../include/gemm.h"
 
@@ -30,7 +38,7 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int MAX_K = 131071;      // 128 * 128 * MAX_K < 2^31
+constexpr int MAX_K = 131071;  // 128 * 128 * MAX_K < 2^31
 constexpr int CHUNK = 16;
 
 struct I8Args {
@@ -39,7 +47,9 @@ struct I8Args {
     char *C;
     long long lda, ldb, ldc;
     int M, N, K, tiles_m, tiles_n;
-    long long first;
+    int span;   // K of a workgroup (a multiple of 128), or all of it
+    int *part;  // span < K: (ranges of K, M, N) sums
+    long long part_stride;
 };
 
 template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int BK_>
@@ -138,7 +148,8 @@ struct Operands {
     i32x4 a[FM], b[FN];
 };
 
-template <typename Tile, typename T>
+// T: of C, or int for sums of a range of K. PAST: stores go past the L2 caches.
+template <typename Tile, typename T, bool PAST>
 __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     constexpr int BM = Tile::BM, BN = Tile::BN, BK = Tile::BK, FM = Tile::FM, FN = Tile::FN;
     // Objects of their own, so that reads of one stage do not wait for the
@@ -146,10 +157,12 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     __shared__ __attribute__((aligned(256))) char a0[BM * BK], a1[BM * BK], a2[BM * BK];
     __shared__ __attribute__((aligned(256))) char b0[BN * BK], b1[BN * BK];
     int tm, tn;
-    group_tile(xcd_remap((int)blockIdx.x, (int)gridDim.x), a.tiles_m, a.tiles_n, 8, tm, tn);
+    const int tiles = a.tiles_m * a.tiles_n, range = blockIdx.x / tiles;
+    group_tile(xcd_remap((int)blockIdx.x - range * tiles, tiles), a.tiles_m, a.tiles_n, 8, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const __amdgpu_buffer_rsrc_t A = operand(a.A + (long long)m0 * a.lda);
-    const __amdgpu_buffer_rsrc_t B = operand(a.B + (long long)n0 * a.ldb);
+    const int from = range * a.span, K = min(a.span, a.K - from);
+    const __amdgpu_buffer_rsrc_t A = operand(a.A + m0 * a.lda + from);
+    const __amdgpu_buffer_rsrc_t B = operand(a.B + n0 * a.ldb + from);
     Staging<BM, Tile::NT, BK> sa;
     Staging<BN, Tile::NT, BK> sb;
     sa.setup(a.M - m0, (int)a.lda);
@@ -170,14 +183,14 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     // Operands of one step of 32 k, and of the next while it is multiplied.
     typedef Operands<FM, FN> Step;
     Step even, odd;
-    const int last = (a.K - 1) / CHUNK * CHUNK;
+    const int last = (K - 1) / CHUNK * CHUNK;
     constexpr int LA = decltype(sa)::LOADS, LB = decltype(sb)::LOADS;
     // Load i of a pair of stages: of B's stage kb into lb, then of A's stage ka into la.
     const auto load = [&](char *la, int ka, char *lb, int kb, int i) {
         if (i < LB) {
-            if (kb < a.K) sb.load(B, lb, kb, last, i);
+            if (kb < K) sb.load(B, lb, kb, last, i);
         } else {
-            if (ka < a.K) sa.load(A, la, ka, last, i - LB);
+            if (ka < K) sa.load(A, la, ka, last, i - LB);
         }
     };
     // Read i of a step's operands, in the order in which the products want them.
@@ -228,7 +241,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
         // This wave has read the stage, and its loads of the next are in LDS (A's of
         // the one behind it may be on their way); behind the barrier everybody's are.
         __builtin_amdgcn_s_waitcnt(0x0070 | LA);  // vmcnt(LA), lgkmcnt(0)
-        if (k0 + 2 * BK >= a.K) __builtin_amdgcn_s_waitcnt(0x0070);
+        if (k0 + 2 * BK >= K) __builtin_amdgcn_s_waitcnt(0x0070);
         barrier();
         step(odd, even, na, nb, 0, la, k0 + 3 * BK, lb, k0 + 2 * BK, 0, L0);
     };
@@ -251,7 +264,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (a.K > 0) {
+    if (K > 0) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) load(a0, 0, b0, 0, i);
 #pragma unroll
@@ -260,12 +273,12 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
         for (int i = 0; i < L0; ++i) load(a2, 2 * BK, b1, BK, i);
         static_assert(L0 <= LB, "the loads behind the first two stages' A are B's");
         __builtin_amdgcn_s_waitcnt(0x0f70 | (LA + L0));
-        if (a.K <= 2 * BK) __builtin_amdgcn_s_waitcnt(0x0f70);
+        if (K <= 2 * BK) __builtin_amdgcn_s_waitcnt(0x0f70);
         barrier();
 #pragma unroll
         for (int i = 0; i < FM + FN; ++i) read(even, a0, b0, 0, i);
         int k0 = 0;
-        for (; k0 + 6 * BK < a.K; k0 += 6 * BK) {
+        for (; k0 + 6 * BK < K; k0 += 6 * BK) {
             stage(a2, b1, a0, b0, a1, b1, k0);
             stage(a0, b0, a1, b1, a2, b0, k0 + BK);
             stage(a1, b1, a2, b0, a0, b1, k0 + 2 * BK);
@@ -273,7 +286,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
             stage(a0, b1, a1, b0, a2, b1, k0 + 4 * BK);
             stage(a1, b0, a2, b1, a0, b0, k0 + 5 * BK);
         }
-        rest = a.K - k0;
+        rest = K - k0;
         const char *la = a0, *lb = b0;
         const auto left = [&](const char *na, const char *nb) {
             rest -= BK;
@@ -302,8 +315,10 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
 
     // Lane: column l % 32 of C, rows 8 g + 4 (l / 32) + 0..3 in registers 4 g + 0..3:
     // a store fills 32 columns of two rows. Rows are uniform but for half.
-    const unsigned sub = 4u * half * (unsigned)a.ldc + r;
+    const long long ldc = std::is_same_v<T, int> ? (long long)a.N : a.ldc;
+    const unsigned sub = 4u * half * (unsigned)ldc + r;
     const bool inside = m0 + BM <= a.M && n0 + BN <= a.N;
+    constexpr bool PART = std::is_same_v<T, int>;
     // The scales by LDS, whose stages have been read: loads from memory there would
     // wait for the stores before them.
     float *scale_m = (float *)a0, *scale_n = scale_m + BM, *bias_n = scale_n + BN;
@@ -318,7 +333,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
         sn[j] = scale_n[wn + j * 32 + r];
         bias[j] = bias_n[wn + j * 32 + r];
     }
-    T *row = (T *)a.C + (m0 + wm) * a.ldc + (n0 + wn);
+    T *row = (T *)(PART ? (char *)(a.part + range * a.part_stride) : a.C) + (m0 + wm) * ldc + (n0 + wn);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -331,35 +346,203 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
                 if (inside || m < a.M) {
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
-                        if (inside || n0 + wn + j * 32 + r < a.N)
-                            row[sub + j * 32] = (T)__builtin_fmaf(
-                                (float)acc[i][j][4 * g + e] * each[e], sn[j], bias[j]);
+                        if (inside || n0 + wn + j * 32 + r < a.N) {
+                            const int sum = acc[i][j][4 * g + e];
+                            const T y =
+                                PART ? (T)sum
+                                     : (T)__builtin_fmaf((float)sum * each[e], sn[j], bias[j]);
+                            if (PAST)
+                                __builtin_nontemporal_store(y, row + sub + j * 32);
+                            else
+                                row[sub + j * 32] = y;
+                        }
                 }
-                row += e == 3 ? 5 * a.ldc : a.ldc;
-                // (one row after the other: all rows' addresses at once do not fit the registers)
+                row += e == 3 ? 5 * ldc : ldc;
+                // (row by row: all rows' addresses at once do not fit the registers)
                 asm volatile("" : "+s"(row));
             }
         }
 }
 
+// Few rows: bound by the weights' bytes and by latency. A workgroup takes 16
+// columns, each of its waves a range of K, and no stage passes through LDS: a
+// wave's loads are the operands of v_mfma_i32_16x16x64_i8 (lane l: 16 bytes of
+// row l % 16 at k = 16 (l / 16)), several on their way at once. The waves' sums
+// meet in LDS. 1 x 16384 x 16384 49.5 us, 5.4 TB/s, the rate of a copy.
+template <int FM, typename T>
+__global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a) {
+    extern __shared__ i32x4 sums[];  // (waves, FM, 64 lanes)
+    constexpr int UNIT = 64, AHEAD = 4;
+    const int lane = threadIdx.x & 63, r = lane & 15, quarter = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6;
+    const int n0 = blockIdx.x * 16;
+    const int units = (a.K + UNIT - 1) / UNIT, last = (a.K - 1) / CHUNK * CHUNK;
+    const int first = (int)((long long)units * wave / waves);
+    const int end = (int)((long long)units * (wave + 1) / waves);
+    const signed char *A[FM], *B = a.B + min(n0 + r, a.N - 1) * a.ldb;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) A[i] = a.A + min(16 * i + r, a.M - 1) * a.lda;
+
+    i32x4 acc[FM] = {};
+    for (int u = first; u < end; u += AHEAD) {
+        i32x4 fa[AHEAD][FM], fb[AHEAD];
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) {
+            if (u + x >= end) break;
+            const int k = min((u + x) * UNIT + quarter * CHUNK, last);
+            fb[x] = *(const i32x4 *)(B + k);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[x][i] = *(const i32x4 *)(A[i] + k);
+        }
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) {
+            if (u + x >= end) break;
+            if ((u + x + 1) * UNIT > a.K) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    fa[x][i] = first_bytes(fa[x][i], a.K - (u + x) * UNIT - quarter * CHUNK);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+                acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[x][i], fb[x], acc[i], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sums[(wave * FM + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    // Register e of lane l is row 4 (l / 16) + e, column l % 16 of its block.
+    const int *part = (const int *)sums;
+    for (int at = threadIdx.x; at < FM * 256; at += blockDim.x) {
+        const int m = at / 16, c = at % 16, n = n0 + c;
+        if (m >= a.M || n >= a.N) continue;
+        const int from = (m / 16 * 64 + (m % 16 / 4) * 16 + c) * 4 + m % 4;
+        int sum = 0;
+        for (int w = 0; w < waves; ++w) sum += part[w * FM * 256 + from];
+        const float y = (float)sum * a.a_scales[m];
+        ((T *)a.C)[m * a.ldc + n] = (T)__builtin_fmaf(y, a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
+    }
+}
+
+template <int FM, typename T>
+void launch_few(I8Args &a, hipStream_t stream) {
+    // Three units of K a wave, up to 16 waves (1 x 50257 x 768: one unit 12.1 us,
+    // three 8.5).
+    const int waves = std::min(16, std::max(1, ceil_div(ceil_div(a.K, 64), 3)));
+    launch(i8_few_kernel<FM, T>, dim3(ceil_div(a.N, 16)), dim3(64 * waves),
+           waves * FM * 64 * sizeof(i32x4), stream, a);
+}
+
+// C from the sums of the ranges of K: four results a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void i8_join_kernel(I8Args a, int ranges, FastDiv columns) {
+    const long long all = (long long)a.M * a.N;
+    const long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (first >= all) return;
+    i32x4 sum = *(const i32x4 *)(a.part + first);
+    for (int x = 1; x < ranges; ++x) sum += *(const i32x4 *)(a.part + x * a.part_stride + first);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (first + e >= all) return;
+        const int m = columns.quot((int)(first + e)), n = (int)(first + e) - m * a.N;
+        const float y = (float)sum[e] * a.a_scales[m];
+        ((T *)a.C)[m * a.ldc + n] = (T)__builtin_fmaf(y, a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
+    }
+}
+
+// What the L2 caches of the eight XCDs hold together.
+constexpr long long L2_BYTES = 32 << 20;
+
+// How a product is cut. tile: an index below; ranges: of K.
+struct I8Plan {
+    int tile, ranges, span;
+};
+
 template <typename Tile, typename T>
-void launch_tile(I8Args &a, hipStream_t stream) {
+void launch_tile(I8Args &a, int ranges, hipStream_t stream) {
     a.tiles_m = ceil_div(a.M, Tile::BM);
     a.tiles_n = ceil_div(a.N, Tile::BN);
-    launch(i8_kernel<Tile, T>, dim3((long long)a.tiles_m * a.tiles_n), dim3(Tile::NT), 0, stream, a);
+    const dim3 grid(a.tiles_m * a.tiles_n * ranges);
+    if (ranges == 1) {
+        // Results that do not fit the L2 caches are stored past them where every
+        // store fills whole lines (8192 x 6400 x 1600 in fp16: 131 -> 115 us;
+        // where rows are odd, 1000 x 50257 x 768 in fp32, it would be 99 -> 117).
+        const bool past = (long long)a.M * a.N * (int)sizeof(T) > L2_BYTES && a.ldc % 32 == 0 &&
+                          (uintptr_t)a.C % (32 * sizeof(T)) == 0;
+        launch(past ? i8_kernel<Tile, T, true> : i8_kernel<Tile, T, false>, grid, dim3(Tile::NT), 0,
+               stream, a);
+        return;
+    }
+    launch(i8_kernel<Tile, int, false>, grid, dim3(Tile::NT), 0, stream, a);
+    launch(i8_join_kernel<T>, dim3((unsigned)(((long long)a.M * a.N + 1023) / 1024)), dim3(256), 0,
+           stream, a, ranges, FastDiv::of(a.N));
+}
+
+enum { FEW, TILE_64, TILE_128, TILE_256, TILE_OUT };
+
+// The rule, with times in us of 16-bit results (FEW, 64 x 64 ranges of K in
+// parentheses, 128 x 128, 256 x 256, 128 x 256 in stages of 64):
+//   1 x 768 x 6400          5.8  11.8 (8: 8.0)  18    50   50
+//   32 x 4096 x 4096        8.4  14.3 (4: 9.8)  19    35   36
+//   32 x 16384 x 1600      10.3   8.7           12    19   19
+//   64 x 4096 x 4096             14.5 (4: 10)   20    37   38
+//   256 x 768 x 6400             20.8 (8: 11)   28    56   57
+//   512 x 4096 x 4096            16.3           21    40   38
+//   1024 x 4096 x 4096           27.6           23    41   39
+//   2048 x 4096 x 4096           53             38    43   46
+//   8192 x 2304 x 768            31.5           29    35   29
+//   1000 x 50257 x 768          103             93    88   79
+//   8192 x 6400 x 1600          166            134   115  132
+//   8192 x 1600 x 6400          128             95    82  102
+// A tile has to leave few CUs idle, a larger one reads less; with few k the
+// results' bytes count, and workgroups that overlap others' stores.
+I8Plan plan_of(int M, int N, int K) {
+    I8Plan p = {TILE_64, 1, K};
+    const auto tiles = [&](long long bm, long long bn) {
+        return (M + bm - 1) / bm * ((N + bn - 1) / bn);
+    };
+    // The share of 256 CUs that whole rounds of 256 x 256 tiles keep busy.
+    const long long t256 = tiles(256, 256);
+    const bool full = t256 * 10 >= (t256 + 255) / 256 * 256 * 7;
+    const int stages = std::max(1, ceil_div(K, 128));
+    if (M <= 32 && (N <= 8192 || K > 8192)) {
+        p.tile = FEW;
+    } else if (K < 1024 && tiles(128, 256) >= 512) {
+        p.tile = TILE_OUT;
+    } else if (full && K >= 1024) {
+        p.tile = TILE_256;
+    } else if (M > 64 && tiles(128, 128) >= 192) {
+        p.tile = TILE_128;
+    } else {
+        // Few tiles of many k: two workgroups a CU, ranges of at least six stages.
+        const long long t64 = tiles(64, 64);
+        const int ranges = (int)std::min(511 / std::max(1ll, t64), stages / 6ll);
+        if (ranges > 1 && stages >= 16) {
+            p.span = ceil_div(stages, ranges) * 128;
+            p.ranges = ceil_div(K, p.span);
+        }
+    }
+    return p;
 }
 
 template <typename T>
-void launch_i8(I8Args &a, hipStream_t stream) {
-    const auto tiles = [&](long long bm, long long bn) {
-        return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn);
-    };
-    if (tiles(256, 256) >= 256)
-        launch_tile<I8Tile<256, 256, 2, 4, 128>, T>(a, stream);
-    else if (tiles(128, 128) >= 256)
-        launch_tile<I8Tile<128, 128, 2, 2, 128>, T>(a, stream);
+void launch_i8(I8Args &a, const I8Plan &p, hipStream_t stream) {
+    a.span = p.span;
+    a.part_stride = ((long long)a.M * a.N + 3) / 4 * 4;
+    if (p.tile == FEW)
+        a.M <= 16 ? launch_few<1, T>(a, stream) : launch_few<2, T>(a, stream);
+    else if (p.tile == TILE_64)
+        launch_tile<I8Tile<64, 64, 2, 2, 128>, T>(a, p.ranges, stream);
+    else if (p.tile == TILE_128)
+        launch_tile<I8Tile<128, 128, 2, 2, 128>, T>(a, p.ranges, stream);
+    else if (p.tile == TILE_256)
+        launch_tile<I8Tile<256, 256, 2, 4, 128>, T>(a, p.ranges, stream);
     else
-        launch_tile<I8Tile<64, 64, 2, 2, 128>, T>(a, stream);
+        launch_tile<I8Tile<128, 256, 2, 4, 64>, T>(a, p.ranges, stream);
+}
+
+size_t bytes_of(const I8Plan &p, int M, int N) {
+    return p.ranges == 1 ? 0 : ((size_t)M * N + 3) / 4 * 4 * sizeof(int) * p.ranges;
 }
 
 const char *size_fault(const GemmI8 *g) {
@@ -377,7 +560,11 @@ const char *size_fault(const GemmI8 *g) {
 
 extern "C" {
 
-size_t gemm_i8_workspace(const GemmI8 *g) { return 0; }
+size_t gemm_i8_workspace(const GemmI8 *g) {
+    using namespace bmb;
+    if (size_fault(g) || g->M == 0 || g->N == 0) return 0;
+    return bytes_of(plan_of(g->M, g->N, g->K), g->M, g->N);
+}
 
 int gemm_i8(const GemmI8 *g, hipStream_t stream) {
     using namespace bmb;
@@ -394,7 +581,7 @@ int gemm_i8(const GemmI8 *g, hipStream_t stream) {
              (unsigned long long)g->ldb) % 16 != 0)
             return refuse(me, "A, B or their strides are no multiples of 16 bytes");
     }
-    if (g->ldc < g->N || g->ldc > (1ll << 40)) return refuse(me, "ldc is below N or above 2^40");
+    if (g->ldc < g->N || g->ldc >= (1 << 30)) return refuse(me, "ldc is below N or not below 2^30");
     if ((uintptr_t)g->C % size != 0 ||
         ((uintptr_t)g->a_scales | (uintptr_t)g->b_scales | (uintptr_t)g->bias) % 4 != 0)
         return refuse(me, "a buffer is no multiple of its element's size");
@@ -407,14 +594,38 @@ int gemm_i8(const GemmI8 *g, hipStream_t stream) {
     if (clash(g->A, M, g->lda, g->K) || clash(g->B, N, g->ldb, g->K) ||
         clash(g->a_scales, M, 4, 4) || clash(g->b_scales, N, 4, 4) || clash(g->bias, N, 4, 4))
         return refuse(me, "C overlaps an input");
-    I8Args a = {g->A, g->B, g->a_scales, g->b_scales, g->bias, (char *)g->C, g->lda, g->ldb,
-                g->ldc, g->M, g->N, g->K, 0, 0, 0};
-    if (g->type == BMB_F32)
-        launch_i8<float>(a, stream);
-    else if (g->type == BMB_F16)
-        launch_i8<_Float16>(a, stream);
-    else
-        launch_i8<__bf16>(a, stream);
+    I8Plan plan = plan_of(g->M, g->N, g->K);
+    const size_t need = bytes_of(plan, g->M, g->N);
+    if (g->work != nullptr && need > 0) {
+        if (g->work_bytes < need) return refuse(me, "the workspace is too small");
+        if ((uintptr_t)g->work % 16 != 0)
+            return refuse(me, "the workspace is no multiple of 16 bytes");
+        if (clash(g->work, 1, 0, need)) return refuse(me, "C overlaps the workspace");
+    }
+    const auto go = [&](void *work) {
+        I8Args a = {g->A, g->B, g->a_scales, g->b_scales, g->bias, (char *)g->C, g->lda, g->ldb,
+                    g->ldc, g->M, g->N, g->K, 0, 0, 0, (int *)work, 0};
+        if (g->type == BMB_F32)
+            launch_i8<float>(a, plan, stream);
+        else if (g->type == BMB_F16)
+            launch_i8<_Float16>(a, plan, stream);
+        else
+            launch_i8<__bf16>(a, plan, stream);
+    };
+    if (need == 0 || g->work != nullptr) {
+        go(g->work);
+        return 0;
+    }
+    if (!stream_capturing(stream)) {
+        ScratchLease ws(SCRATCH_GEMM, need, stream);
+        if (ws) {
+            go(ws.get());
+            return 0;
+        }
+    }
+    plan.ranges = 1;
+    plan.span = g->K;
+    go(nullptr);
     return 0;
 }
 

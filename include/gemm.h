@@ -101,10 +101,12 @@ int gemm_get_math(void);
  *     C[m,n] = (sum_k A[m,k] * B[n,k]) * a_scales[m] * b_scales[n] + bias[n]
  * The sum is exact (whole numbers in 32 bits, so K is at most 131071). It is
  * rounded to fp32, so is its product with a_scales[m], and so is that product's
- * with b_scales[n] together with the bias; the result is rounded to `type`. A, B and their strides are multiples of 16
- * bytes; K is any number: what a row holds behind it has no influence, but up
- * to the next multiple of 16 it is read. C needs its element's alignment;
- * what lies between its rows is left as it was. C overlaps nothing else. */
+ * with b_scales[n] together with the bias; the result is rounded to `type`. A, B
+ * and their strides are multiples of 16 bytes; K is any number: what a row holds
+ * behind it has no influence, but up to the next multiple of 16 it is read. C
+ * needs its element's alignment (ldc a multiple of 32 and C of 128 bytes are
+ * fastest where it is large); what lies between its rows is left as it was. C
+ * overlaps nothing else. */
 typedef struct GemmI8 {
     int M, N, K;
     int type; /* of C: BMB_F32 0, BMB_F16 1 or BMB_BF16 2 (nn.h) */
@@ -112,7 +114,7 @@ typedef struct GemmI8 {
     const float *a_scales, *b_scales; /* (M), (N) */
     const float *bias;                /* (N), or null */
     void *C;                          /* (M, N) */
-    long long lda, ldb, ldc;          /* elements from row to row; lda and ldb below 2^23 */
+    long long lda, ldb, ldc; /* elements from row to row; lda, ldb below 2^23, ldc below 2^30 */
     void *work;                       /* device memory, used by one call at a time */
     size_t work_bytes;
 } GemmI8;

@@ -228,8 +228,9 @@ typedef struct Rotary {
 #define BMB_ROTARY_UNSCALED 0 /* as they are */
 #define BMB_ROTARY_LINEAR 1   /* / factor */
 #define BMB_ROTARY_BASE 2     /* of base * factor^(dims / (dims - 2)) (dims 2: as they are) */
-#define BMB_ROTARY_PARTS 3    /* those that turn slow times or less over trained_len positions: / factor; */
-                              /* fast times or more: as they are; between: evenly from one to the other */
+#define BMB_ROTARY_PARTS 3    /* those that turn `slow` times or less over trained_len */
+                              /* positions: / factor; `fast` times or more: as they are; */
+                              /* between: evenly from the one to the other */
 /* Fills plan->freq on the host; launches nothing. factor >= 1; trained_len,
  * slow and fast (0 <= slow < fast) are looked at for BMB_ROTARY_PARTS only. */
 int rotary_frequencies(Rotary *plan, double base, int scaling, double factor, int trained_len,
