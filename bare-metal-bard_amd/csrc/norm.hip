@@ -3,9 +3,13 @@
 // three).
 //
 // All of them are bound by HBM: a row is read once, kept in registers across
-// its reduction, and written once. G threads share a row (a wave, four or
-// sixteen), each with P pieces of 16 bytes. Rows wider than the registers of
-// 1024 threads take kernels that read them twice.
+// its reduction, and written once. G threads share a row (one, four, eight or
+// sixteen waves), each with P pieces of 16 bytes, at most 16 elements, so that
+// enough rows are on their way. Rows of more than 16384 take kernels that read
+// them twice. At 5.15 TB/s, the rate of a copy: 8192 x 768 in fp32 with residual and
+// sum 21.6 us (floor 19.6), its backward 23 (19.6; the next row is loaded while
+// one is reduced, without that 28), 16381 x 4096 in bf16 112 (104), 50257 x 768 in
+// fp32 to 8 bits 40 (37.5).
 //
 // The mean of the squares is held in 64 bits, and so are the products of the
 // result: squares of fp32 numbers pass fp32's range, and so can rstd (1 ULP of
@@ -57,6 +61,19 @@ __device__ __forceinline__ void load_piece(const T *row, int c, int C, float (&v
         for (int e = 0; e < N; ++e) v[e] = c + e < C ? (float)row[c + e] : 0.0f;
     }
 }
+// The same as they are.
+template <typename T, int N>
+__device__ __forceinline__ Piece<T, N> load_raw(const T *row, int c, int C) {
+    Piece<T, N> x = {};
+    if (c + N <= C) {
+        x = *(const typename Unaligned<T, N>::type *)(row + c);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (c + e < C) x[e] = row[c + e];
+    }
+    return x;
+}
 template <typename T, int N, typename V>
 __device__ __forceinline__ void store_piece(T *row, int c, int C, const V (&v)[N]) {
     if (c + N <= C) {
@@ -71,12 +88,38 @@ __device__ __forceinline__ void store_piece(T *row, int c, int C, const V (&v)[N
     }
 }
 
-// f over the 64 lanes, the result in each.
+// The value of another lane of the DPP row or row group, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float from_lane(float x) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double x) {
+    const int2 v = __builtin_bit_cast(int2, x);
+    return __builtin_bit_cast(
+        double, make_int2(__builtin_amdgcn_update_dpp(0, v.x, CTRL, ROWS, 0xf, false),
+                          __builtin_amdgcn_update_dpp(0, v.y, CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float last_lane(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ double last_lane(double x) {
+    const int2 v = __builtin_bit_cast(int2, x);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(v.x, 63),
+                                                __builtin_amdgcn_readlane(v.y, 63)));
+}
+// f, for which 0 changes nothing, over the 64 lanes: inside rows of 16 lanes,
+// then from row to row into lane 63, and to all.
 template <typename V, typename F>
 __device__ __forceinline__ V wave_all(V x, F &&f) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x = f(x, __shfl_xor(x, d));
-    return x;
+    x = f(x, from_lane<0x111, 0xf>(x));
+    x = f(x, from_lane<0x112, 0xf>(x));
+    x = f(x, from_lane<0x114, 0xf>(x));
+    x = f(x, from_lane<0x118, 0xf>(x));
+    x = f(x, from_lane<0x142, 0xa>(x));
+    x = f(x, from_lane<0x143, 0xc>(x));
+    return last_lane(x);
 }
 // f over the G threads of a row (G = 64, or the whole workgroup), in a fixed
 // order.
@@ -314,42 +357,50 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void grad_kernel(GradArgs a) {
 #pragma unroll
         for (int e = 0; e < N; ++e) dw[i][e] = 0.0f;
     }
-    for (long long row = first + lane_row; row < last; row += ROWS) {
+    // The next row's pieces are on their way while a row is reduced (1024 threads
+    // have no registers for that).
+    constexpr bool AHEAD = G < 1024;
+    Piece<T, N> dr[P], xr[P], gr[P] = {};
+    float rstd_next = 0.0f;
+    const auto fetch = [&](long long row) {
+        if (row >= last) return;
         const T *dout = (const T *)a.dout + row * a.dout_stride;
         const T *inp = (const T *)a.inp + row * a.inp_stride;
-        const float rstd = a.rstd[row];
-        float d[P][N], xhat[P][N], dot = 0.0f;
+        const T *dres = (const T *)a.dres + row * a.dres_stride;
+        rstd_next = a.rstd[row];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int c = (i * G + t) * N;
-            load_piece<T, N>(dout, c, a.C, d[i]);
-            load_piece<T, N>(inp, c, a.C, xhat[i]);
+            dr[i] = load_raw<T, N>(dout, c, a.C);
+            xr[i] = load_raw<T, N>(inp, c, a.C);
+            if (a.dres) gr[i] = load_raw<T, N>(dres, c, a.C);
         }
+    };
+    if (AHEAD) fetch(first + lane_row);
+    for (long long row = first + lane_row; row < last; row += ROWS) {
+        if (!AHEAD) fetch(row);
+        const float rstd = rstd_next;
+        float d[P][N], xhat[P][N], g[P][N], dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < P; ++i)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                xhat[i][e] *= rstd;
+                d[i][e] = (float)dr[i][e];
+                xhat[i][e] = (float)xr[i][e] * rstd;
+                g[i][e] = (float)gr[i][e];
                 dw[i][e] = __builtin_fmaf(d[i][e], xhat[i][e], dw[i][e]);
                 d[i][e] *= w[i][e];
                 dot = __builtin_fmaf(d[i][e], xhat[i][e], dot);
             }
+        if (AHEAD) fetch(row + ROWS);
         dot = row_all<G>(dot, part, Add()) / a.C;
         T *dinp = (T *)a.dinp + row * a.dinp_stride;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int c = (i * G + t) * N;
-            float g[N];
-            if (a.dres) {
-                load_piece<T, N>((const T *)a.dres + row * a.dres_stride, c, a.C, g);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) g[e] = 0.0f;
-            }
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                g[e] += rstd * __builtin_fmaf(-xhat[i][e], dot, d[i][e]);
-            store_piece<T, N>(dinp, c, a.C, g);
+                g[i][e] += rstd * __builtin_fmaf(-xhat[i][e], dot, d[i][e]);
+            store_piece<T, N>(dinp, (i * G + t) * N, a.C, g[i]);
         }
     }
     if (!a.part) return;
@@ -427,51 +478,70 @@ __global__ __launch_bounds__(256) void wide_sums_kernel(GradArgs a) {
     store_piece<float, N>(a.part + block * a.C, c, a.C, dw);
 }
 
-// dweight += the workgroups' sums, in their order, in 64 bits.
-__global__ __launch_bounds__(256) void join_sums_kernel(float *dweight, const float *part,
-                                                        int blocks, int C) {
+// dweight += the workgroups' sums, in a fixed order, in 64 bits: 16 columns a
+// workgroup, 256 rows of sums at once.
+__global__ __launch_bounds__(1024) void join_sums_kernel(float *dweight, const float *part,
+                                                         int blocks, int C) {
     __shared__ double lds[16][16];
-    const int x = threadIdx.x % 16, y = threadIdx.x / 16, c = blockIdx.x * 16 + x;
-    double s = 0.0;
-    if (c < C)
-        for (int b = y; b < blocks; b += 16) s += part[(size_t)b * C + c];
-    lds[y][x] = s;
+    const int x = threadIdx.x % 4 * 4, y = threadIdx.x / 4, c = blockIdx.x * 16 + x;
+    const int column = blockIdx.x * 16 + threadIdx.x;
+    const float before = threadIdx.x < 16 && column < C ? dweight[column] : 0.0f;
+    double s[4] = {};
+    for (int b = y; b < blocks; b += 256) {
+        float v[4];
+        load_piece<float, 4>(part + (long long)b * C, c, C, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int d = 32; d > 2; d >>= 1) s[e] += __shfl_xor(s[e], d);
+        if ((threadIdx.x & 63) < 4) lds[threadIdx.x >> 6][x + e] = s[e];
+    }
     __syncthreads();
-    if (y == 0 && c < C) {
-        for (int i = 1; i < 16; ++i) s += lds[i][x];
-        dweight[c] = (float)(dweight[c] + s);
+    if (threadIdx.x < 16 && column < C) {
+        double sum = before;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += lds[i][threadIdx.x];
+        dweight[column] = (float)sum;
     }
 }
 
-// Threads of a row and pieces of each; G = 0: the wide kernels.
+// Threads of a row and pieces of each, at most `elements` a thread; G = 0: the
+// wide kernels.
 struct Shape {
     int G, P;
 };
-Shape shape_of(int C, int size) {
-    const int pieces = ceil_div(C, 16 / size);
-    for (int G : {64, 256, 1024})
-        if (pieces <= 4 * G) return {G, ceil_div(pieces, G)};
+Shape shape_of(int C, int size, int elements) {
+    const int pieces = ceil_div(C, 16 / size), most = elements * size / 16;
+    for (int G : {64, 256, 512, 1024})
+        if (pieces <= most * G) return {G, ceil_div(pieces, G)};
     return {0, 0};
 }
 
-// f.template operator()<G, P>() for a shape.
-template <int G, typename F>
+// f(G, P) as constants, for P up to MOST.
+template <int MOST, int G, typename F>
 void with_pieces(int P, F &&f) {
-    if (P == 1) f(std::integral_constant<int, G>(), std::integral_constant<int, 1>());
-    else if (P == 2) f(std::integral_constant<int, G>(), std::integral_constant<int, 2>());
-    else if (P == 3) f(std::integral_constant<int, G>(), std::integral_constant<int, 3>());
-    else f(std::integral_constant<int, G>(), std::integral_constant<int, 4>());
+    if constexpr (MOST > 0) {
+        if (P == MOST)
+            f(std::integral_constant<int, G>(), std::integral_constant<int, MOST>());
+        else
+            with_pieces<MOST - 1, G>(P, f);
+    }
 }
-template <typename F>
+template <int MOST, typename F>
 void with_shape(Shape s, F &&f) {
-    if (s.G == 64) with_pieces<64>(s.P, f);
-    else if (s.G == 256) with_pieces<256>(s.P, f);
-    else with_pieces<1024>(s.P, f);
+    if (s.G == 64) with_pieces<MOST, 64>(s.P, f);
+    else if (s.G == 256) with_pieces<MOST, 256>(s.P, f);
+    else if (s.G == 512) with_pieces<MOST, 512>(s.P, f);
+    else with_pieces<MOST, 1024>(s.P, f);
 }
 
 template <typename T, bool NORM, bool I8>
 void launch_rows(NormArgs &a, hipStream_t stream) {
-    const Shape s = shape_of(a.C, sizeof(T));
+    constexpr int MOST = 16 / piece_of<T>();  // 16 elements a thread
+    const Shape s = shape_of(a.C, sizeof(T), 16);
     const auto go = [&](auto kernel, int threads, int rows_each) {
         in_launches(((long long)a.rows + rows_each - 1) / rows_each, threads,
                     [&](long long first, unsigned n) {
@@ -482,8 +552,9 @@ void launch_rows(NormArgs &a, hipStream_t stream) {
     if (s.G == 0)
         go(wide_rows_kernel<T, NORM, I8>, 1024, 1);
     else
-        with_shape(s, [&](auto G, auto P) {
-            go(rows_kernel<T, NORM, I8, G(), P()>, std::max(256, (int)G), G() < 256 ? 256 / G() : 1);
+        with_shape<MOST>(s, [&](auto G, auto P) {
+            go(rows_kernel<T, NORM, I8, G(), P()>, std::max(256, (int)G),
+               G() < 256 ? 256 / G() : 1);
         });
 }
 
@@ -493,14 +564,18 @@ struct Spans {
 };
 Spans spans_of(int rows) {
     Spans s;
-    s.span = std::min(64, std::max(4, (int)((rows + 1023ll) / 1024)));
+    // Two workgroups a CU (16381 x 4096 in bf16, where each is four times as wide:
+    // one 104 us, two 108, four 116; 8192 x 768 in fp32: 20.8, 18.5 and 19.8), and
+    // at most 64 rows.
+    s.span = (int)std::min(64ll, std::max(4ll, (rows + 511ll) / 512));
     s.blocks = (int)((rows + s.span - 1ll) / s.span);
     return s;
 }
 
 template <typename T>
 void launch_grad(GradArgs &a, hipStream_t stream) {
-    const Shape s = shape_of(a.C, sizeof(T));
+    constexpr int MOST = 16 / piece_of<T>();  // 16 elements a thread
+    const Shape s = shape_of(a.C, sizeof(T), 16);
     const Spans n = spans_of(a.rows);
     a.span = n.span;
     const auto go = [&](auto kernel, long long blocks, int threads, size_t lds) {
@@ -514,7 +589,7 @@ void launch_grad(GradArgs &a, hipStream_t stream) {
         if (a.part) go(wide_sums_kernel<T>, chunks * n.blocks, 256, 0);
         go(wide_grad_kernel<T>, a.rows, 1024, 0);
     } else {
-        with_shape(s, [&](auto G, auto P) {
+        with_shape<MOST>(s, [&](auto G, auto P) {
             const size_t lds = G() < 256 ? (size_t)a.C * (256 / G()) * sizeof(float) : 0;
             go(grad_kernel<T, G(), P()>, n.blocks, std::max(256, (int)G), lds);
         });
@@ -680,7 +755,7 @@ int rms_norm_backward(const RmsNormGrad *g, hipStream_t stream) {
         else
             launch_grad<__bf16>(a, stream);
         if (part)
-            launch(join_sums_kernel, dim3(ceil_div(g->C, 16)), dim3(256), 0, stream, g->dweight,
+            launch(join_sums_kernel, dim3(ceil_div(g->C, 16)), dim3(1024), 0, stream, g->dweight,
                    part, spans_of(g->rows).blocks, g->C);
     };
     if (need == 0) {
