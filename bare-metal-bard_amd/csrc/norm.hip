@@ -568,7 +568,7 @@ Spans spans_of(int rows) {
     // one 104 us, two 108, four 116; 8192 x 768 in fp32: 20.8, 18.5 and 19.8), and
     // at most 64 rows.
     s.span = (int)std::min(64ll, std::max(4ll, (rows + 511ll) / 512));
-    s.blocks = (int)((rows + s.span - 1ll) / s.span);
+    s.blocks = (int)(((long long)rows + s.span - 1) / s.span);
     return s;
 }
 
