@@ -5,16 +5,16 @@
 // both supply the same k in the same place, their order inside the instruction
 // does not matter. Sums are whole numbers in 32 bits: exact, in any order.
 //
-// A stage is 128 k (64 where few k leave the results' bytes the bound). Its tile
-// of A and of B goes from global memory straight into LDS (16 bytes a lane, no
-// registers). LDS holds three stages of A and two of B (all 160 KB for 256 x 256
-// tiles): what bounds a tile is how long before its use a load is issued. In
-// steps of 32 k a wave multiplies what it has read, and between the products
-// reads the next step's operands and issues loads; one barrier a stage. 8192^3
-// (256 x 256 tiles): two stages of both, all loads at the stage's start 525 us;
-// spread 510; scales by LDS instead of from memory between the stores, which
-// waited for the stores, 477; A three stages deep 446 (2470 TOP/s; on zeros
-// 365: the matrix cores run at 1.7 of 2.4 GHz, held back by power).
+// A stage is 128 k. Its tile of A and of B goes from global memory straight into
+// LDS (16 bytes a lane, no registers). LDS holds three stages of A and two of B
+// (all 160 KB for 256 x 256 tiles): what bounds a tile is how long before its use a
+// load is issued. In steps of 32 k a wave multiplies what it has read, and between
+// the products reads the next step's operands and issues loads; one barrier a
+// stage. 8192^3 (256 x 256 tiles): two stages of both, all loads at the stage's
+// start 525 us; spread 510; scales by LDS instead of from memory between the
+// stores, which waited for the stores, 477; A three stages deep 446; results by
+// LDS in whole rows 429 (2560 TOP/s; the matrix cores are busy two thirds of the
+// time at 1.7 of 2.4 GHz: power bounds the clock).
 //
 // Edges. Rows past the last are loaded from the last one and reach only
 // results that are not stored. In a last stage that is not whole, chunks past
@@ -39,7 +39,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int MAX_K = 131071;  // 128 * 128 * MAX_K < 2^31
-constexpr int CHUNK = 16;
+constexpr int BK = 128, STEPS = BK / 32;  // k of a stage, and steps of 32 k
+constexpr int CHUNK = 16, CHUNKS = BK / CHUNK;
 
 struct I8Args {
     const signed char *A, *B;
@@ -52,45 +53,34 @@ struct I8Args {
     long long part_stride;
 };
 
-template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int BK_>
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_>
 struct I8Tile {
-    static constexpr int BM = BM_, BN = BN_, BK = BK_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
+    static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
     static constexpr int NT = 64 * WAVES_M * WAVES_N;
     static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 32, FN = WN / 32;
 };
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-// A stage's rows in LDS: BK bytes, their 16-byte chunks permuted by the row so
+// A stage's rows in LDS: 128 bytes, their 16-byte chunks permuted by the row so
 // that the groups of 16 lanes in which a 128-bit read of 32 rows is served, {0-3,
 // 12-15, 20-27}, {4-11, 16-19, 28-31}, touch 16 different places modulo 256
-// bytes. Rows of 64 bytes also swap places in pairs.
-template <int BK>
-struct Layout {
-    static constexpr int CHUNKS = BK / CHUNK;
-    static_assert(BK == 64 || BK == 128, "the permutations are these two's");
-    __device__ static __forceinline__ int slot(int row) {  // of a row (and row of a slot)
-        return BK == 64 ? row ^ ((row >> 2) & 1) : row;
-    }
-    __device__ static __forceinline__ int permuted(int row, int chunk) {
-        return chunk ^ (BK == 64 ? (row >> 3) & 3 : (row >> 1) & 7);
-    }
-};
+// bytes (no bank conflict is counted).
+__device__ __forceinline__ int permuted(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
 
 // ROWS rows of one operand's stage into LDS: lane i of a wave fills the i-th
-// chunk of 1 KB; the workgroup's load i rows i * STEP on, where rows and chunks
-// are permuted alike (STEP is a multiple of 32).
-template <int ROWS, int NT, int BK>
+// chunk of 1 KB, eight rows; the workgroup's load i rows i * STEP on, where
+// chunks are permuted alike (STEP is a multiple of 16).
+template <int ROWS, int NT>
 struct Staging {
-    typedef Layout<BK> L;
-    static constexpr int LOADS = ROWS * L::CHUNKS / NT, STEP = NT / L::CHUNKS;
-    static_assert(STEP % 32 == 0, "permutations depend on the row modulo 32");
+    static constexpr int LOADS = ROWS * CHUNKS / NT, STEP = NT / CHUNKS;
+    static_assert(STEP % 16 == 0, "permutations depend on the row modulo 16");
     int row, chunk;      // byte offsets of this lane's first row, and in it
     int step, last_row;  // of the next load's row, and of the operand's last row
     __device__ __forceinline__ void setup(int rows, int ld) {
-        const int slot = threadIdx.x / L::CHUNKS, r = L::slot(slot);
+        const int r = threadIdx.x / CHUNKS;
         row = r * ld;
-        chunk = L::permuted(r, threadIdx.x % L::CHUNKS) * CHUNK;
+        chunk = permuted(r, threadIdx.x % CHUNKS) * CHUNK;
         step = STEP * ld;
         last_row = (min(rows, ROWS) - 1) * ld;
     }
@@ -114,11 +104,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t operand(const signed char *p) 
 
 // Where this lane finds its operand of a stage's first step in row r of the
 // tile; those of step kk are at place ^ 32 kk, and of rows 32 i on 32 i rows on.
-template <int BK>
 __device__ __forceinline__ int place_of(int r, int half) {
-    return Layout<BK>::slot(r) * BK + Layout<BK>::permuted(r, half) * CHUNK;
+    return r * BK + permuted(r, half) * CHUNK;
 }
-template <int BK>
 __device__ __forceinline__ i32x4 operand_at(const char *lds, int place, int kk, int i) {
     return *(const i32x4 *)(lds + ((place ^ (32 * kk)) + i * 32 * BK));
 }
@@ -142,6 +130,13 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
+// xcd_remap() for any number of workgroups: XCD x, which is given ids x, x + 8,
+// ..., takes consecutive tiles.
+__device__ __forceinline__ int xcd_order(int id, int blocks) {
+    const int x = id % 8, each = blocks / 8, more = blocks % 8;
+    return x * each + min(x, more) + id / 8;
+}
+
 // A wave's operands of one step of 32 k.
 template <int FM, int FN>
 struct Operands {
@@ -151,20 +146,20 @@ struct Operands {
 // T: of C, or int for sums of a range of K. PAST: stores go past the L2 caches.
 template <typename Tile, typename T, bool PAST>
 __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
-    constexpr int BM = Tile::BM, BN = Tile::BN, BK = Tile::BK, FM = Tile::FM, FN = Tile::FN;
+    constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN;
     // Objects of their own, so that reads of one stage do not wait for the
     // loads into the other.
     __shared__ __attribute__((aligned(256))) char a0[BM * BK], a1[BM * BK], a2[BM * BK];
     __shared__ __attribute__((aligned(256))) char b0[BN * BK], b1[BN * BK];
     int tm, tn;
     const int tiles = a.tiles_m * a.tiles_n, range = blockIdx.x / tiles;
-    group_tile(xcd_remap((int)blockIdx.x - range * tiles, tiles), a.tiles_m, a.tiles_n, 8, tm, tn);
+    group_tile(xcd_order((int)blockIdx.x - range * tiles, tiles), a.tiles_m, a.tiles_n, 8, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int from = range * a.span, K = min(a.span, a.K - from);
     const __amdgpu_buffer_rsrc_t A = operand(a.A + m0 * a.lda + from);
     const __amdgpu_buffer_rsrc_t B = operand(a.B + n0 * a.ldb + from);
-    Staging<BM, Tile::NT, BK> sa;
-    Staging<BN, Tile::NT, BK> sb;
+    Staging<BM, Tile::NT> sa;
+    Staging<BN, Tile::NT> sb;
     sa.setup(a.M - m0, (int)a.lda);
     sb.setup(a.N - n0, (int)a.ldb);
     static_assert(BM <= Tile::NT && BN <= Tile::NT, "a scale a thread");
@@ -177,7 +172,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     const int wm = wave / Tile::WAVES_N * Tile::WM, wn = wave % Tile::WAVES_N * Tile::WN;
     const int r = lane & 31, half = lane >> 5;
 
-    int place_a = place_of<BK>(wm + r, half), place_b = place_of<BK>(wn + r, half);
+    int place_a = place_of(wm + r, half), place_b = place_of(wn + r, half);
 
     i32x16 acc[FM][FN] = {};
     // Operands of one step of 32 k, and of the next while it is multiplied.
@@ -196,9 +191,9 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     // Read i of a step's operands, in the order in which the products want them.
     const auto read = [&](Step &f, const char *la, const char *lb, int kk, int i) {
         if (i == 0 || i > FN)
-            f.a[i ? i - FN : 0] = operand_at<BK>(la, place_a, kk, i ? i - FN : 0);
+            f.a[i ? i - FN : 0] = operand_at(la, place_a, kk, i ? i - FN : 0);
         else
-            f.b[i - 1] = operand_at<BK>(lb, place_b, kk, i - 1);
+            f.b[i - 1] = operand_at(lb, place_b, kk, i - 1);
     };
     const auto product = [&](const Step &f, int t) {
         const int i = t / FN, j = t % FN;
@@ -229,15 +224,12 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     // L0 in the last step, the others in the next stage, whose `la` and `lb` before
     // are pa, pb) are spread over the steps: a wave that issues them all at once
     // waits until the memory pipeline has taken them.
-    constexpr int STEPS = BK / 32, LOADS = LA + LB, L0 = (3 * LOADS + 7) / 8;
-    constexpr int L1 = STEPS == 2 ? LOADS - L0 : L0, L2 = LOADS - L0 - L1;
+    constexpr int LOADS = LA + LB, L0 = (3 * LOADS + 7) / 8, L1 = L0, L2 = LOADS - L0 - L1;
     const auto stage = [&](char *pa, char *pb, char *la, char *lb, const char *na, const char *nb,
                            int k0) {
         step(even, odd, la, lb, 1, pa, k0 + 2 * BK, pb, k0 + BK, L0, L1);
-        if constexpr (STEPS == 4) {
-            step(odd, even, la, lb, 2, pa, k0 + 2 * BK, pb, k0 + BK, L0 + L1, L2);
-            step(even, odd, la, lb, 3, pa, 0, pb, 0, 0, 0);
-        }
+        step(odd, even, la, lb, 2, pa, k0 + 2 * BK, pb, k0 + BK, L0 + L1, L2);
+        step(even, odd, la, lb, 3, pa, 0, pb, 0, 0, 0);
         // This wave has read the stage, and its loads of the next are in LDS (A's of
         // the one behind it may be on their way); behind the barrier everybody's are.
         __builtin_amdgcn_s_waitcnt(0x0070 | LA);  // vmcnt(LA), lgkmcnt(0)
@@ -313,53 +305,69 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
         finish(la, lb);
     }
 
-    // Lane: column l % 32 of C, rows 8 g + 4 (l / 32) + 0..3 in registers 4 g + 0..3:
-    // a store fills 32 columns of two rows. Rows are uniform but for half.
-    const long long ldc = std::is_same_v<T, int> ? (long long)a.N : a.ldc;
-    const unsigned sub = 4u * half * (unsigned)ldc + r;
-    const bool inside = m0 + BM <= a.M && n0 + BN <= a.N;
+    // Results leave by LDS, eight rows of each wave row at a time, in two places in
+    // turn: lane l has column l % 32, rows 8 g + 4 (l / 32) + 0..3 of a 32 x 32 block
+    // in registers 4 g + 0..3; a lane then stores four columns of a row, so that
+    // a store takes 256 columns in a piece, wherever rows begin. The scales come
+    // by LDS too: loads from memory would wait for the stores before them.
     constexpr bool PART = std::is_same_v<T, int>;
-    // The scales by LDS, whose stages have been read: loads from memory there would
-    // wait for the stores before them.
+    typedef std::conditional_t<PART, int, float> V;
+    constexpr int ROWS = Tile::WAVES_M * 8, LINE = BN / 4;  // lanes of a row
+    static_assert(ROWS * BN * 4 <= BN * BK && (BM + 2 * BN) * 4 <= BM * BK, "they fit the stages");
     float *scale_m = (float *)a0, *scale_n = scale_m + BM, *bias_n = scale_n + BN;
-    __syncthreads();
+    __syncthreads();  // the stages have been read
     if (tid < BM) scale_m[tid] = scale_of_m;
     if (tid < BN) scale_n[tid] = scale_of_n;
     if (tid < BN) bias_n[tid] = bias_of_n;
     __syncthreads();
+    const long long ldc = PART ? (long long)a.N : a.ldc;
+    T *C = (T *)(PART ? (char *)(a.part + range * a.part_stride) : a.C) + n0;
     float sn[FN], bias[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         sn[j] = scale_n[wn + j * 32 + r];
         bias[j] = bias_n[wn + j * 32 + r];
     }
-    T *row = (T *)(PART ? (char *)(a.part + range * a.part_stride) : a.C) + (m0 + wm) * ldc + (n0 + wn);
+    // (rows 4..7 of eight move by 32 columns: both halves of a wave write at once)
+    const auto at = [](int row, int c) { return row * BN + (c ^ ((row & 4) << 3)); };
+    const int columns = min(BN, a.N - n0);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
+            V *place = (V *)((i * 4 + g) % 2 ? b1 : b0);
             const float4 sm = *(const float4 *)(scale_m + wm + i * 32 + 8 * g + 4 * half);
             const float each[4] = {sm.x, sm.y, sm.z, sm.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int m = m0 + wm + i * 32 + 8 * g + e + 4 * half;
-                if (inside || m < a.M) {
+            for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int j = 0; j < FN; ++j)
-                        if (inside || n0 + wn + j * 32 + r < a.N) {
-                            const int sum = acc[i][j][4 * g + e];
-                            const T y =
-                                PART ? (T)sum
-                                     : (T)__builtin_fmaf((float)sum * each[e], sn[j], bias[j]);
-                            if (PAST)
-                                __builtin_nontemporal_store(y, row + sub + j * 32);
-                            else
-                                row[sub + j * 32] = y;
-                        }
+                for (int e = 0; e < 4; ++e) {
+                    const int sum = acc[i][j][4 * g + e];
+                    place[at(wm / Tile::WM * 8 + 4 * half + e, wn + j * 32 + r)] =
+                        PART ? (V)sum : (V)__builtin_fmaf((float)sum * each[e], sn[j], bias[j]);
                 }
-                row += e == 3 ? 5 * ldc : ldc;
-                // (row by row: all rows' addresses at once do not fit the registers)
-                asm volatile("" : "+s"(row));
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+            barrier();
+#pragma unroll
+            for (int x = 0; x < ROWS * LINE / Tile::NT; ++x) {
+                const int t = x * Tile::NT + tid, row = t / LINE, c = t % LINE * 4;
+                const int m = m0 + row / 8 * Tile::WM + i * 32 + 8 * g + row % 8;
+                typedef V V4 __attribute__((ext_vector_type(4)));
+                const V4 v = *(const V4 *)(place + at(row, c));
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                typedef T4 Unaligned __attribute__((aligned(sizeof(T))));
+                const T4 y = __builtin_convertvector(v, T4);
+                T *to = C + m * ldc + c;
+                if (m < a.M && c + 4 <= columns) {
+                    if (PAST)
+                        __builtin_nontemporal_store(y, (Unaligned *)to);
+                    else
+                        *(Unaligned *)to = y;
+                } else if (m < a.M) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < columns) to[e] = y[e];
+                }
             }
         }
 }
@@ -464,11 +472,9 @@ void launch_tile(I8Args &a, int ranges, hipStream_t stream) {
     a.tiles_n = ceil_div(a.N, Tile::BN);
     const dim3 grid(a.tiles_m * a.tiles_n * ranges);
     if (ranges == 1) {
-        // Results that do not fit the L2 caches are stored past them where every
-        // store fills whole lines (8192 x 6400 x 1600 in fp16: 131 -> 115 us;
-        // where rows are odd, 1000 x 50257 x 768 in fp32, it would be 99 -> 117).
-        const bool past = (long long)a.M * a.N * (int)sizeof(T) > L2_BYTES && a.ldc % 32 == 0 &&
-                          (uintptr_t)a.C % (32 * sizeof(T)) == 0;
+        // Results that do not fit the L2 caches are stored past them (1000 x 50257 x
+        // 768 in fp32: 94 -> 86 us).
+        const bool past = (long long)a.M * a.N * (int)sizeof(T) > L2_BYTES;
         launch(past ? i8_kernel<Tile, T, true> : i8_kernel<Tile, T, false>, grid, dim3(Tile::NT), 0,
                stream, a);
         return;
@@ -478,24 +484,23 @@ void launch_tile(I8Args &a, int ranges, hipStream_t stream) {
            stream, a, ranges, FastDiv::of(a.N));
 }
 
-enum { FEW, TILE_64, TILE_128, TILE_256, TILE_OUT };
+enum { FEW, TILE_64, TILE_128, TILE_256 };
 
-// The rule, with times in us of 16-bit results (FEW, 64 x 64 ranges of K in
-// parentheses, 128 x 128, 256 x 256, 128 x 256 in stages of 64):
-//   1 x 768 x 6400          5.8  11.8 (8: 8.0)  18    50   50
-//   32 x 4096 x 4096        8.4  14.3 (4: 9.8)  19    35   36
-//   32 x 16384 x 1600      10.3   8.7           12    19   19
-//   64 x 4096 x 4096             14.5 (4: 10)   20    37   38
-//   256 x 768 x 6400             20.8 (8: 11)   28    56   57
-//   512 x 4096 x 4096            16.3           21    40   38
-//   1024 x 4096 x 4096           27.6           23    41   39
-//   2048 x 4096 x 4096           53             38    43   46
-//   8192 x 2304 x 768            31.5           29    35   29
-//   1000 x 50257 x 768          103             93    88   79
-//   8192 x 6400 x 1600          166            134   115  132
-//   8192 x 1600 x 6400          128             95    82  102
-// A tile has to leave few CUs idle, a larger one reads less; with few k the
-// results' bytes count, and workgroups that overlap others' stores.
+// The rule, with times in us of 16-bit results (FEW; 64 x 64, ranges of K in
+// parentheses; 128 x 128; 256 x 256):
+//   1 x 768 x 6400          5.8  11.8 (8: 8.0)  18    50
+//   32 x 4096 x 4096        8.4  14.3 (4: 9.8)  19    35
+//   32 x 16384 x 1600      10.3   8.7           12    19
+//   64 x 4096 x 4096             14.5 (4: 10)   20    37
+//   256 x 768 x 6400             20.8 (8: 11)   28    56
+//   512 x 4096 x 4096            16.2           21    40
+//   1024 x 4096 x 4096           27.5           22    39
+//   2048 x 4096 x 4096           52             37    41
+//   8192 x 2304 x 768            29             26    30
+//   1000 x 50257 x 768           88             76    72
+//   8192 x 6400 x 1600          159            109   105
+//   8192 x 1600 x 6400          128             95    82
+// A tile has to leave few CUs idle; a larger one reads less.
 I8Plan plan_of(int M, int N, int K) {
     I8Plan p = {TILE_64, 1, K};
     const auto tiles = [&](long long bm, long long bn) {
@@ -507,9 +512,7 @@ I8Plan plan_of(int M, int N, int K) {
     const int stages = std::max(1, ceil_div(K, 128));
     if (M <= 32 && (N <= 8192 || K > 8192)) {
         p.tile = FEW;
-    } else if (K < 1024 && tiles(128, 256) >= 512) {
-        p.tile = TILE_OUT;
-    } else if (full && K >= 1024) {
+    } else if (M > 64 && full) {
         p.tile = TILE_256;
     } else if (M > 64 && tiles(128, 128) >= 192) {
         p.tile = TILE_128;
@@ -532,13 +535,11 @@ void launch_i8(I8Args &a, const I8Plan &p, hipStream_t stream) {
     if (p.tile == FEW)
         a.M <= 16 ? launch_few<1, T>(a, stream) : launch_few<2, T>(a, stream);
     else if (p.tile == TILE_64)
-        launch_tile<I8Tile<64, 64, 2, 2, 128>, T>(a, p.ranges, stream);
+        launch_tile<I8Tile<64, 64, 2, 2>, T>(a, p.ranges, stream);
     else if (p.tile == TILE_128)
-        launch_tile<I8Tile<128, 128, 2, 2, 128>, T>(a, p.ranges, stream);
-    else if (p.tile == TILE_256)
-        launch_tile<I8Tile<256, 256, 2, 4, 128>, T>(a, p.ranges, stream);
+        launch_tile<I8Tile<128, 128, 2, 2>, T>(a, p.ranges, stream);
     else
-        launch_tile<I8Tile<128, 256, 2, 4, 64>, T>(a, p.ranges, stream);
+        launch_tile<I8Tile<256, 256, 2, 4>, T>(a, p.ranges, stream);
 }
 
 size_t bytes_of(const I8Plan &p, int M, int N) {
