@@ -6,15 +6,16 @@
 // does not matter. Sums are whole numbers in 32 bits: exact, in any order.
 //
 // A stage is 128 k. Its tile of A and of B goes from global memory straight into
-// LDS (16 bytes a lane, no registers). LDS holds three stages of A and two of B
-// (all 160 KB for 256 x 256 tiles): what bounds a tile is how long before its use a
-// load is issued. In steps of 32 k a wave multiplies what it has read, and between
-// the products reads the next step's operands and issues loads; one barrier a
-// stage. 8192^3 (256 x 256 tiles): two stages of both, all loads at the stage's
-// start 525 us; spread 510; scales by LDS instead of from memory between the
-// stores, which waited for the stores, 477; A three stages deep 446; results by
-// LDS in whole rows 429 (2560 TOP/s; the matrix cores are busy two thirds of the
-// time at 1.7 of 2.4 GHz: power bounds the clock).
+// LDS (16 bytes a lane, no registers). LDS holds three stages of A and two or
+// three of B (all 160 KB for 256 x 256 tiles): what bounds a tile is how long
+// before its use a load is issued. In steps of 32 k a wave multiplies what it has
+// read, and between the products reads the next step's operands and issues loads;
+// one barrier a stage. 8192^3 (256 x 256 tiles): two stages of both, all loads at
+// the stage's start 525 us; spread 510; scales by LDS instead of from memory
+// between the stores, which waited for the stores, 477; A three stages deep 446;
+// results by LDS in whole rows 429; no wait in the loop but for the next stage 423
+// (2600 TOP/s; the matrix cores are busy two thirds of the time at 1.7 of 2.4 GHz:
+// power bounds the clock).
 //
 // Edges. Rows past the last are loaded from the last one and reach only
 // results that are not stored. In a last stage that is not whole, chunks past
@@ -53,8 +54,10 @@ struct I8Args {
     long long part_stride;
 };
 
-template <int BM_, int BN_, int WAVES_M_, int WAVES_N_>
+// DA, DB: stages of A and of B in LDS.
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int DA_, int DB_>
 struct I8Tile {
+    static constexpr int DA = DA_, DB = DB_;
     static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
     static constexpr int NT = 64 * WAVES_M * WAVES_N;
     static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 32, FN = WN / 32;
@@ -121,6 +124,18 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 x, int n) {
     return x;
 }
 
+// f(0), ..., f(N - 1) as constants.
+template <int N, typename F>
+__device__ __forceinline__ void for_each(F &&f) {
+    if constexpr (N > 0) {
+        for_each<N - 1>(f);
+        f(std::integral_constant<int, N - 1>());
+    }
+}
+
+// s_waitcnt's operand: at most n loads from memory on their way, whatever else.
+constexpr int vmcnt(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
+
 // A barrier that waits for nothing but the other waves (__syncthreads() also
 // waits for every load into LDS that is on its way). The caller has waited for
 // what the others will read.
@@ -149,8 +164,16 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN;
     // Objects of their own, so that reads of one stage do not wait for the
     // loads into the other.
+    constexpr int DA = Tile::DA, DB = Tile::DB;
+    static_assert(DA == 3 && (DB == 2 || DB == 3), "stages in LDS");
     __shared__ __attribute__((aligned(256))) char a0[BM * BK], a1[BM * BK], a2[BM * BK];
     __shared__ __attribute__((aligned(256))) char b0[BN * BK], b1[BN * BK];
+    char *b2 = nullptr;
+    if constexpr (DB == 3) {
+        __shared__ __attribute__((aligned(256))) char more[BN * BK];
+        b2 = more;
+    }
+    char *const as[3] = {a0, a1, a2}, *const bs[3] = {b0, b1, b2};
     int tm, tn;
     const int tiles = a.tiles_m * a.tiles_n, range = blockIdx.x / tiles;
     group_tile(xcd_order((int)blockIdx.x - range * tiles, tiles), a.tiles_m, a.tiles_n, 8, tm, tn);
@@ -218,24 +241,26 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Stage k0 in la, lb (the operands of its first step are read) up to the first
-    // step of the next in na, nb. Behind the barrier its places are free for
-    // A's stage after the next two and B's after the next; these loads (the first
-    // L0 in the last step, the others in the next stage, whose `la` and `lb` before
-    // are pa, pb) are spread over the steps: a wave that issues them all at once
-    // waits until the memory pipeline has taken them.
+    // Stage k0, the i-th, in its places (the operands of its first step are read), up
+    // to the first step of the next. Behind the barrier its places are free for A's
+    // stage DA and B's stage DB after it; these loads (the first L0 in the last step,
+    // the others in the next stage) are spread over the steps: a wave that issues
+    // them all at once waits until the memory pipeline has taken them.
     constexpr int LOADS = LA + LB, L0 = (3 * LOADS + 7) / 8, L1 = L0, L2 = LOADS - L0 - L1;
-    const auto stage = [&](char *pa, char *pb, char *la, char *lb, const char *na, const char *nb,
-                           int k0) {
-        step(even, odd, la, lb, 1, pa, k0 + 2 * BK, pb, k0 + BK, L0, L1);
-        step(odd, even, la, lb, 2, pa, k0 + 2 * BK, pb, k0 + BK, L0 + L1, L2);
+    // Loads that may be on their way when the next stage has to be there.
+    constexpr int LATER = (DA - 2) * LA + (DB - 2) * LB;
+    const auto stage = [&](int i, int k0) {
+        char *la = as[i % DA], *lb = bs[i % DB], *pa = as[(i + DA - 1) % DA];
+        char *pb = bs[(i + DB - 1) % DB], *na = as[(i + 1) % DA], *nb = bs[(i + 1) % DB];
+        step(even, odd, la, lb, 1, pa, k0 + (DA - 1) * BK, pb, k0 + (DB - 1) * BK, L0, L1);
+        step(odd, even, la, lb, 2, pa, k0 + (DA - 1) * BK, pb, k0 + (DB - 1) * BK, L0 + L1, L2);
         step(even, odd, la, lb, 3, pa, 0, pb, 0, 0, 0);
-        // This wave has read the stage, and its loads of the next are in LDS (A's of
-        // the one behind it may be on their way); behind the barrier everybody's are.
-        __builtin_amdgcn_s_waitcnt(0x0070 | LA);  // vmcnt(LA), lgkmcnt(0)
-        if (k0 + 2 * BK >= K) __builtin_amdgcn_s_waitcnt(0x0070);
+        // This wave has read the stage, and its loads of the next are in LDS; behind
+        // the barrier everybody's are. (The last stages have fewer loads behind them.)
+        __builtin_amdgcn_s_waitcnt(vmcnt(LATER) & 0xf0ff);  // and lgkmcnt(0)
+        if (k0 + (DA - 1) * BK >= K) __builtin_amdgcn_s_waitcnt(vmcnt(0));
         barrier();
-        step(odd, even, na, nb, 0, la, k0 + 3 * BK, lb, k0 + 2 * BK, 0, L0);
+        step(odd, even, na, nb, 0, la, k0 + DA * BK, lb, k0 + DB * BK, 0, L0);
     };
     // The last stage, of `rest` k.
     int rest = 0;
@@ -258,50 +283,38 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
     };
     if (K > 0) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) load(a0, 0, b0, 0, i);
+        for (int x = 0; x < DA - 1; ++x) {
 #pragma unroll
-        for (int i = LB; i < LOADS; ++i) load(a1, BK, b1, BK, i);
+            for (int i = x < DB - 1 ? 0 : LB; i < LOADS; ++i) load(as[x], x * BK, bs[x], x * BK, i);
+        }
 #pragma unroll
-        for (int i = 0; i < L0; ++i) load(a2, 2 * BK, b1, BK, i);
-        static_assert(L0 <= LB, "the loads behind the first two stages' A are B's");
-        __builtin_amdgcn_s_waitcnt(0x0f70 | (LA + L0));
-        if (K <= 2 * BK) __builtin_amdgcn_s_waitcnt(0x0f70);
+        for (int i = 0; i < L0; ++i)
+            load(as[DA - 1], (DA - 1) * BK, bs[DB - 1], (DB - 1) * BK, i);
+        static_assert(L0 <= LB, "these are B's");
+        __builtin_amdgcn_s_waitcnt(vmcnt(LATER + L0));
+        if (K <= (DA - 1) * BK) __builtin_amdgcn_s_waitcnt(vmcnt(0));
         barrier();
 #pragma unroll
         for (int i = 0; i < FM + FN; ++i) read(even, a0, b0, 0, i);
+        // As many stages as bring every one back to its places.
+        constexpr int TURN = DA == DB ? DA : DA * DB;
         int k0 = 0;
-        for (; k0 + 6 * BK < K; k0 += 6 * BK) {
-            stage(a2, b1, a0, b0, a1, b1, k0);
-            stage(a0, b0, a1, b1, a2, b0, k0 + BK);
-            stage(a1, b1, a2, b0, a0, b1, k0 + 2 * BK);
-            stage(a2, b0, a0, b1, a1, b0, k0 + 3 * BK);
-            stage(a0, b1, a1, b0, a2, b1, k0 + 4 * BK);
-            stage(a1, b0, a2, b1, a0, b0, k0 + 5 * BK);
-        }
+        for (; k0 + (TURN + DA - 1) * BK < K; k0 += TURN * BK)
+            for_each<TURN>([&](auto i) { stage(i(), k0 + i() * BK); });
         rest = K - k0;
         const char *la = a0, *lb = b0;
-        const auto left = [&](const char *na, const char *nb) {
-            rest -= BK;
-            la = na;
-            lb = nb;
-            return rest > BK;
-        };
-        if (rest > BK) {
-            stage(a2, b1, a0, b0, a1, b1, k0);
-            if (left(a1, b1)) {
-                stage(a0, b0, a1, b1, a2, b0, k0 + BK);
-                if (left(a2, b0)) {
-                    stage(a1, b1, a2, b0, a0, b1, k0 + 2 * BK);
-                    if (left(a0, b1)) {
-                        stage(a2, b0, a0, b1, a1, b0, k0 + 3 * BK);
-                        if (left(a1, b0)) {
-                            stage(a0, b1, a1, b0, a2, b1, k0 + 4 * BK);
-                            left(a2, b1);
-                        }
-                    }
-                }
+        const auto left = [&](auto self, auto number) {
+            constexpr int i = decltype(number)::value;
+            if constexpr (i + 1 < TURN + DA) {
+                if (rest <= BK) return;
+                stage(i, k0 + i * BK);
+                rest -= BK;
+                la = as[(i + 1) % DA];
+                lb = bs[(i + 1) % DB];
+                self(self, std::integral_constant<int, i + 1>());
             }
-        }
+        };
+        left(left, std::integral_constant<int, 0>());
         finish(la, lb);
     }
 
@@ -464,6 +477,7 @@ constexpr long long L2_BYTES = 32 << 20;
 // How a product is cut. tile: an index below; ranges: of K.
 struct I8Plan {
     int tile, ranges, span;
+    bool deep;
 };
 
 template <typename Tile, typename T>
@@ -486,23 +500,28 @@ void launch_tile(I8Args &a, int ranges, hipStream_t stream) {
 
 enum { FEW, TILE_64, TILE_128, TILE_256 };
 
-// The rule, with times in us of 16-bit results (FEW; 64 x 64, ranges of K in
+// The rule, with times in us of 16-bit results (few rows; 64 x 64, ranges of K in
 // parentheses; 128 x 128; 256 x 256):
-//   1 x 768 x 6400          5.8  11.8 (8: 8.0)  18    50
-//   32 x 4096 x 4096        8.4  14.3 (4: 9.8)  19    35
-//   32 x 16384 x 1600      10.3   8.7           12    19
-//   64 x 4096 x 4096             14.5 (4: 10)   20    37
-//   256 x 768 x 6400             20.8 (8: 11)   28    56
-//   512 x 4096 x 4096            16.2           21    40
-//   1024 x 4096 x 4096           27.5           22    39
-//   2048 x 4096 x 4096           52             37    41
-//   8192 x 2304 x 768            29             26    30
+//   1 x 768 x 6400          5.8  (4: 8.5)
+//   32 x 2304 x 768         3.9   4.2 (2: 6.3)
+//   32 x 4096 x 4096        8.4  10.0 (2: 9.4)
+//   32 x 8192 x 768         5.1   4.3 (2: 6.5)
+//   32 x 4096 x 16384      24.9  29.4 (4: 16.1)
+//   1 x 16384 x 16384      49.8  59.6 (8: 57.7)
+//   64 x 4096 x 4096             10.3 (2: 9.8, 4: 9.8)
+//   128 x 1600 x 4800            12.2 (4: 9.4)
+//   256 x 768 x 6400             14.0 (4: 9.9)
+//   512 x 1600 x 6400            14.4 (2: 16.2)
+//   512 x 4096 x 4096            14.9           21    40
+//   1024 x 4096 x 4096           27.5           20    39
+//   2048 x 4096 x 4096           52             36    41
+//   8192 x 2304 x 768            29             25    30
 //   1000 x 50257 x 768           88             76    72
-//   8192 x 6400 x 1600          159            109   105
-//   8192 x 1600 x 6400          128             95    82
+//   8192 x 6400 x 1600          159            109   102
+//   8192 x 1600 x 6400          128             95    80
 // A tile has to leave few CUs idle; a larger one reads less.
 I8Plan plan_of(int M, int N, int K) {
-    I8Plan p = {TILE_64, 1, K};
+    I8Plan p = {TILE_64, 1, K, false};
     const auto tiles = [&](long long bm, long long bn) {
         return (M + bm - 1) / bm * ((N + bn - 1) / bn);
     };
@@ -510,21 +529,27 @@ I8Plan plan_of(int M, int N, int K) {
     const long long t256 = tiles(256, 256);
     const bool full = t256 * 10 >= (t256 + 255) / 256 * 256 * 7;
     const int stages = std::max(1, ceil_div(K, 128));
-    if (M <= 32 && (N <= 8192 || K > 8192)) {
+    if (N <= 4096 ? M <= 32 && K <= 8192 : M <= 4 && K > 8192) {
         p.tile = FEW;
     } else if (M > 64 && full) {
         p.tile = TILE_256;
     } else if (M > 64 && tiles(128, 128) >= 192) {
         p.tile = TILE_128;
     } else {
-        // Few tiles of many k: two workgroups a CU, ranges of at least six stages.
-        const long long t64 = tiles(64, 64);
-        const int ranges = (int)std::min(511 / std::max(1ll, t64), stages / 6ll);
-        if (ranges > 1 && stages >= 16) {
+        // Few tiles of many k, which make up for a second launch: at most a workgroup
+        // a CU, ranges of at least ten stages.
+        const long long t64 = std::max(1ll, tiles(64, 64));
+        const int ranges = (int)std::min(256 / t64, stages / 10ll);
+        if (ranges > 1 && stages >= 36) {
             p.span = ceil_div(stages, ranges) * 128;
             p.ranges = ceil_div(K, p.span);
         }
     }
+    // A third stage of B hides more of a load's way, where the LDS that it takes
+    // keeps no workgroup from a CU (256 x 4096 x 4096 14.4 -> 10.6 us, 64 x 6400 x 1600
+    // 7.9 -> 6.6, 1024 x 4096 x 4096 21.7 -> 19.7; 16 x 50257 x 768, 786 tiles, it would
+    // be 9.1 -> 10.6, 2048 x 4096 x 4096 36 -> 38).
+    p.deep = p.tile == TILE_64 ? tiles(64, 64) * p.ranges <= 768 : tiles(128, 128) <= 256;
     return p;
 }
 
@@ -535,11 +560,13 @@ void launch_i8(I8Args &a, const I8Plan &p, hipStream_t stream) {
     if (p.tile == FEW)
         a.M <= 16 ? launch_few<1, T>(a, stream) : launch_few<2, T>(a, stream);
     else if (p.tile == TILE_64)
-        launch_tile<I8Tile<64, 64, 2, 2>, T>(a, p.ranges, stream);
+        p.deep ? launch_tile<I8Tile<64, 64, 2, 2, 3, 3>, T>(a, p.ranges, stream)
+               : launch_tile<I8Tile<64, 64, 2, 2, 3, 2>, T>(a, p.ranges, stream);
     else if (p.tile == TILE_128)
-        launch_tile<I8Tile<128, 128, 2, 2>, T>(a, p.ranges, stream);
+        p.deep ? launch_tile<I8Tile<128, 128, 2, 2, 3, 3>, T>(a, p.ranges, stream)
+               : launch_tile<I8Tile<128, 128, 2, 2, 3, 2>, T>(a, p.ranges, stream);
     else
-        launch_tile<I8Tile<256, 256, 2, 4>, T>(a, p.ranges, stream);
+        launch_tile<I8Tile<256, 256, 2, 4, 3, 2>, T>(a, p.ranges, stream);
 }
 
 size_t bytes_of(const I8Plan &p, int M, int N) {

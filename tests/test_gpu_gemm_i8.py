@@ -96,6 +96,35 @@ def test_many_tiles(gpu, M, N, K, name):
     p.check(p.run())
 
 
+@pytest.mark.parametrize("stages", list(range(1, 19)) + [25, 40])
+@pytest.mark.parametrize("M,N", [(16, 48), (70, 80), (33, 50257), (2048, 2048), (2100, 2300),
+                                 (4096, 4096)])
+def test_stages(gpu, M, N, stages):
+    """Every number of stages of 128 k, the last one whole or not, in each tile; the sums against
+    the product in 64 bits on the device."""
+    for K in (128 * stages, 128 * stages - 61):
+        print("stages", M, N, K, flush=True)
+        g = torch.Generator(device="cuda").manual_seed(stages)
+        ld = line(K)
+        A, B = (torch.randint(-128, 128, (r, ld), device="cuda", generator=g, dtype=torch.int8) | 1
+                for r in (M, N))
+        one = torch.ones(max(M, N), device="cuda")
+        C = Rows(M, N, torch.float32)
+        c = bmb.GemmI8(M=M, N=N, K=K, type=bmb.F32, A=A.data_ptr(), B=B.data_ptr(),
+                       a_scales=one.data_ptr(), b_scales=one.data_ptr(), C=C.ptr, lda=ld, ldb=ld,
+                       ldc=N)
+        need = bmb.gemm_i8_workspace(c)
+        work = torch.empty(max(need, 1), device="cuda", dtype=torch.uint8)
+        c.work, c.work_bytes = work.data_ptr() if need else None, need
+        torch.cuda.synchronize()
+        bmb.gemm_i8(c)
+        torch.cuda.synchronize()
+        bmb.check("gemm_i8")
+        # whole numbers below 2^53; rounded to fp32 as the call does
+        want = torch.matmul(A[:, :K].double(), B[:, :K].double().t()).float()
+        assert torch.equal(C.t, want) and C.intact()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 70, 300), (40, 50, 700), (150, 200, 333), (300, 260, 64)])
 @pytest.mark.parametrize("name", list(TYPES))
 def test_strides(gpu, name, M, N, K):

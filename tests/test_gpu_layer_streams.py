@@ -15,7 +15,7 @@ class Calls:
     """One call of each operator, with results of its own; `work`: with workspaces of the
     caller's."""
 
-    def __init__(self, seed, work=True, name="bf16", rows=300, C=1000, M=64, N=400, K=4096):
+    def __init__(self, seed, work=True, name="bf16", rows=300, C=1000, M=64, N=400, K=8192):
         g = torch.Generator(device="cuda").manual_seed(seed)
         kind, t = TYPES[name]
         rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
@@ -41,7 +41,7 @@ class Calls:
                                     dinp=p["dinp"], dinp_stride=C, dweight=p["dweight"])
         A, B = (torch.randint(-127, 128, (r, K), device="cuda", generator=g, dtype=torch.int8)
                 for r in (M, N))
-        sa, sb = torch.rand(M, device="cuda", generator=g), torch.rand(N, device="cuda", generator=g)
+        sa, sb = (torch.rand(r, device="cuda", generator=g) for r in (M, N))
         keep.update(A=A, B=B, sa=sa, sb=sb)
         self.gemm = bmb.GemmI8(M=M, N=N, K=K, type=kind, A=A.data_ptr(), B=B.data_ptr(),
                                a_scales=sa.data_ptr(), b_scales=sb.data_ptr(), C=p["C"], lda=K,
