@@ -136,9 +136,16 @@ __device__ __forceinline__ void for_each(F &&f) {
 // s_waitcnt's operand: at most n loads from memory on their way, whatever else.
 constexpr int vmcnt(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
 
+// Waits until at most n loads from memory are on their way and every access to
+// LDS is done.
+template <int N>
+__device__ __forceinline__ void wait() {
+    asm volatile("" ::: "memory");  // (the compiler moves no access over it)
+    __builtin_amdgcn_s_waitcnt(vmcnt(N) & 0xf0ff);
+}
 // A barrier that waits for nothing but the other waves (__syncthreads() also
-// waits for every load into LDS that is on its way). The caller has waited for
-// what the others will read.
+// waits for every load into LDS, and every store, that is on its way). The
+// caller has waited for what the others will read.
 __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -257,8 +264,8 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
         step(even, odd, la, lb, 3, pa, 0, pb, 0, 0, 0);
         // This wave has read the stage, and its loads of the next are in LDS; behind
         // the barrier everybody's are. (The last stages have fewer loads behind them.)
-        __builtin_amdgcn_s_waitcnt(vmcnt(LATER) & 0xf0ff);  // and lgkmcnt(0)
-        if (k0 + (DA - 1) * BK >= K) __builtin_amdgcn_s_waitcnt(vmcnt(0));
+        wait<LATER>();
+        if (k0 + (DA - 1) * BK >= K) wait<0>();
         barrier();
         step(odd, even, na, nb, 0, la, k0 + DA * BK, lb, k0 + DB * BK, 0, L0);
     };
@@ -291,8 +298,8 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
         for (int i = 0; i < L0; ++i)
             load(as[DA - 1], (DA - 1) * BK, bs[DB - 1], (DB - 1) * BK, i);
         static_assert(L0 <= LB, "these are B's");
-        __builtin_amdgcn_s_waitcnt(vmcnt(LATER + L0));
-        if (K <= (DA - 1) * BK) __builtin_amdgcn_s_waitcnt(vmcnt(0));
+        wait<LATER + L0>();
+        if (K <= (DA - 1) * BK) wait<0>();
         barrier();
 #pragma unroll
         for (int i = 0; i < FM + FN; ++i) read(even, a0, b0, 0, i);
@@ -359,7 +366,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
                     place[at(wm / Tile::WM * 8 + 4 * half + e, wn + j * 32 + r)] =
                         PART ? (V)sum : (V)__builtin_fmaf((float)sum * each[e], sn[j], bias[j]);
                 }
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+            wait<63>();
             barrier();
 #pragma unroll
             for (int x = 0; x < ROWS * LINE / Tile::NT; ++x) {
@@ -628,7 +635,16 @@ int gemm_i8(const GemmI8 *g, hipStream_t stream) {
         if (g->work_bytes < need) return refuse(me, "the workspace is too small");
         if ((uintptr_t)g->work % 16 != 0)
             return refuse(me, "the workspace is no multiple of 16 bytes");
-        if (clash(g->work, 1, 0, need)) return refuse(me, "C overlaps the workspace");
+        const char *w = (const char *)g->work;
+        const auto within = [&](const void *p, long long rows, long long stride, long long width) {
+            const char *in = (const char *)p;
+            return in != nullptr && width > 0 && w < in + ((rows - 1) * stride + width) &&
+                   in < w + need;
+        };
+        if (clash(w, 1, 0, need) || within(g->A, M, g->lda, g->K) ||
+            within(g->B, N, g->ldb, g->K) || within(g->a_scales, M, 4, 4) || within(g->b_scales, N, 4, 4) ||
+            within(g->bias, N, 4, 4))
+            return refuse(me, "the workspace overlaps another buffer");
     }
     const auto go = [&](void *work) {
         I8Args a = {g->A, g->B, g->a_scales, g->b_scales, g->bias, (char *)g->C, g->lda, g->ldb,

@@ -144,6 +144,29 @@ def test_gemm_refuses(capfd, kw, why):
     refused(capfd, why, bmb.gemm_i8, gemm(**kw))
 
 
+@pytest.mark.parametrize("kw,why", [
+    (dict(work_bytes=16), "too small"), (dict(work=at(6) + 8), "16 bytes"),
+    (dict(work=at(0)), "overlap"), (dict(work=at(1) - 256), "overlap"),
+    (dict(work=at(2)), "overlap"), (dict(work=at(3)), "overlap"), (dict(work=at(4)), "overlap"),
+    (dict(work=at(5)), "overlap")])
+def test_gemm_refuses_workspace(capfd, kw, why):
+    g = gemm(M=64, N=64, K=16384, lda=16384, ldb=16384, ldc=64, work=at(6), work_bytes=1 << 22)
+    need = bmb.gemm_i8_workspace(g)
+    assert 2 * 64 * 64 * 4 <= need <= 1 << 22
+    for k, v in kw.items():
+        setattr(g, k, v)
+    refused(capfd, why, bmb.gemm_i8, g)
+
+
+def test_gemm_workspace():
+    """Only what is split needs one; none for what is refused."""
+    assert bmb.gemm_i8_workspace(gemm()) == 0
+    assert bmb.gemm_i8_workspace(gemm(K=0, A=None, B=None)) == 0
+    assert bmb.gemm_i8_workspace(gemm(M=0, K=16384)) == 0
+    assert bmb.gemm_i8_workspace(gemm(K=131072)) == 0
+    assert bmb.gemm_i8_workspace(gemm(type=7, K=16384)) == 0
+
+
 def rotary(**kw):
     f = dict(head_size=64, dims=64, layout=bmb.ROTARY_HALF, amplitude=1.0)
     f.update(kw)
