@@ -161,8 +161,11 @@ struct Steps {
         if (!plain || fabsf(y - k) > 0.4999f) {
             const double v = (double)s * w;
             // (a is subnormal at the least: the quotient is finite)
-            const double f = plain ? floor((double)y) : fmin(fmax(floor(v / a * 127.0), -127.0), 126.0);
-            const double side = __builtin_fma(-(2.0 * f + 1.0), a, 254.0 * v);
+            const double f =
+                plain ? floor((double)y) : fmin(fmax(floor(v / a * 127.0), -127.0), 126.0);
+            // (254 v takes up to 55 bits: it and what its rounding lost)
+            const double most = 254.0 * v, rest = __builtin_fma(254.0, v, -most);
+            const double side = __builtin_fma(-(2.0 * f + 1.0), a, most) + rest;
             const bool odd = ((int)f & 1) != 0;
             k = (float)(side > 0.0 || (side == 0.0 && odd) ? f + 1.0 : f);
         }

@@ -287,6 +287,29 @@ def test_quantize_half_way(gpu, name, C):
     check_forward(y, w, None, "i8", forward(y, w, None, "i8"))
 
 
+@pytest.mark.parametrize("C", [254, 5000, 17000])
+def test_half_way_products(gpu, C):
+    """Products of 48 bits half-way between two steps, and next to it: 127 m w is the largest, so
+    that (2k + 1) / 2 m w is half-way, which whole numbers tell without a rounding."""
+    print("half-way products", C, flush=True)
+    g = gen(C)
+    m = torch.randint(1 << 14, 1 << 15, (8, 1), generator=g) * 2 + 1
+    odd = torch.arange(C) % 254 * 2 - 253
+    w = (torch.randint(1 << 23, 1 << 24, (1,), generator=g) | 1).expand(C)
+    s = odd * m  # twice the value, so that it is whole
+    s[:, 0] = 254 * m[:, 0]
+    s[4:6, 1:] += 1
+    s[6:8, 1:] -= 1
+    x, weight = s.float() / 2, w.float()
+    assert torch.equal((x.double() * 2).long(), s)
+    O, _, _, _ = forward(x, weight, None, "i8")
+    # q = 127 s / s[0], to the nearest, half-way to the even one
+    num, den = 2 * 127 * s + s[:, :1], 2 * s[:, :1]
+    q = num.div(den, rounding_mode="floor")
+    q -= ((num % den == 0) & (q % 2 != 0)).long()
+    assert torch.equal(O.get().long(), q)
+
+
 def test_quantize_extremes(gpu):
     x = torch.zeros(7, 90)
     x[1] = torch.finfo(torch.float32).max
