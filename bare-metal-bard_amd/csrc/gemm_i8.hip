@@ -14,8 +14,12 @@
 // the stage's start 525 us; spread 510; scales by LDS instead of from memory
 // between the stores, which waited for the stores, 477; A three stages deep 446;
 // results by LDS in whole rows 429; no wait in the loop but for the next stage 423
-// (2600 TOP/s; the matrix cores are busy two thirds of the time at 1.7 of 2.4 GHz:
-// power bounds the clock).
+// (2600 TOP/s; 436-448 on other boxes. The matrix cores are busy 77% of the cycles
+// at about 1.55 of 2.4 GHz: power bounds the clock; on zeros it takes 281).
+// 256 x 256 tiles take a whole CU, so their stores overlap no products: 1000 x 50257 x
+// 768 in fp32 takes 83-88 us, the stores alone 42. 256 x 128 tiles with stages of 64 k,
+// two workgroups a CU, took 71 instead of 79 where rows are whole lines, but 59 instead
+// of 54 for 1024 x 49152 in 16 bits and 581 instead of 435 for 8192^3.
 //
 // Edges. Rows past the last are loaded from the last one and reach only
 // results that are not stored. In a last stage that is not whole, chunks past
@@ -642,8 +646,8 @@ int gemm_i8(const GemmI8 *g, hipStream_t stream) {
                    in < w + need;
         };
         if (clash(w, 1, 0, need) || within(g->A, M, g->lda, g->K) ||
-            within(g->B, N, g->ldb, g->K) || within(g->a_scales, M, 4, 4) || within(g->b_scales, N, 4, 4) ||
-            within(g->bias, N, 4, 4))
+            within(g->B, N, g->ldb, g->K) || within(g->a_scales, M, 4, 4) ||
+            within(g->b_scales, N, 4, 4) || within(g->bias, N, 4, 4))
             return refuse(me, "the workspace overlaps another buffer");
     }
     const auto go = [&](void *work) {

@@ -7,9 +7,9 @@
 // sixteen waves), each with P pieces of 16 bytes, at most 16 elements, so that
 // enough rows are on their way. Rows of more than 16384 take kernels that read
 // them twice. At 5.15 TB/s, the rate of a copy: 8192 x 768 in fp32 with residual and
-// sum 21.6 us (floor 19.6), its backward 23 (19.6; the next row is loaded while
-// one is reduced, without that 28), 16381 x 4096 in bf16 112 (104), 50257 x 768 in
-// fp32 to 8 bits 40 (37.5).
+// sum 21.3 us (floor 19.6), its backward 22.6 (19.6; the next row is loaded while
+// one is reduced, without that 28), 16381 x 4096 in bf16 113 (104), 50257 x 768 in
+// fp32 to 8 bits 39 (37.5).
 //
 // The mean of the squares is held in 64 bits, and so are the products of the
 // result: squares of fp32 numbers pass fp32's range, and so can rstd (1 ULP of
