@@ -163,6 +163,16 @@ __device__ __forceinline__ int xcd_order(int id, int blocks) {
     return x * each + min(x, more) + id / 8;
 }
 
+// A sum's result. (Told nothing, the compiler rounds fp16 results once, of
+// the exact product and sum, where it finds both in one place: the bits would
+// depend on how a product is cut.)
+template <typename T>
+__device__ __forceinline__ T result(int sum, float a_scale, float b_scale, float bias) {
+    float y = __builtin_fmaf((float)sum * a_scale, b_scale, bias);
+    asm("" : "+v"(y));
+    return (T)y;
+}
+
 // A wave's operands of one step of 32 k.
 template <int FM, int FN>
 struct Operands {
@@ -368,7 +378,7 @@ __global__ __launch_bounds__(Tile::NT) void i8_kernel(I8Args a) {
                 for (int e = 0; e < 4; ++e) {
                     const int sum = acc[i][j][4 * g + e];
                     place[at(wm / Tile::WM * 8 + 4 * half + e, wn + j * 32 + r)] =
-                        PART ? (V)sum : (V)__builtin_fmaf((float)sum * each[e], sn[j], bias[j]);
+                        PART ? (V)sum : (V)result<float>(sum, each[e], sn[j], bias[j]);
                 }
             wait<63>();
             barrier();
@@ -451,8 +461,8 @@ __global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a) {
         const int from = (m / 16 * 64 + (m % 16 / 4) * 16 + c) * 4 + m % 4;
         int sum = 0;
         for (int w = 0; w < waves; ++w) sum += part[w * FM * 256 + from];
-        const float y = (float)sum * a.a_scales[m];
-        ((T *)a.C)[m * a.ldc + n] = (T)__builtin_fmaf(y, a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
+        ((T *)a.C)[m * a.ldc + n] =
+            result<T>(sum, a.a_scales[m], a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
     }
 }
 
@@ -477,8 +487,8 @@ __global__ __launch_bounds__(256) void i8_join_kernel(I8Args a, int ranges, Fast
     for (int e = 0; e < 4; ++e) {
         if (first + e >= all) return;
         const int m = columns.quot((int)(first + e)), n = (int)(first + e) - m * a.N;
-        const float y = (float)sum[e] * a.a_scales[m];
-        ((T *)a.C)[m * a.ldc + n] = (T)__builtin_fmaf(y, a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
+        ((T *)a.C)[m * a.ldc + n] =
+            result<T>(sum[e], a.a_scales[m], a.b_scales[n], a.bias ? a.bias[n] : 0.0f);
     }
 }
 

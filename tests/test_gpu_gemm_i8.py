@@ -88,6 +88,22 @@ def test_sizes(gpu, name, M, N, K):
     p.check(p.run())
 
 
+@pytest.mark.parametrize("M,N,K", [(16, 4096, 64), (30, 3000, 200), (64, 1600, 6400), (40, 4100, 96),
+                                   (300, 700, 130), (2100, 2300, 130)])
+@pytest.mark.parametrize("name", list(TYPES))
+def test_roundings(gpu, name, M, N, K):
+    """Without a bias every rounding is known: the sum's, its product's with a_scales, that one's
+    with b_scales, all to fp32, and the result's. To the bit, however the product is cut."""
+    print("roundings", name, M, N, K, flush=True)
+    p = Problem(M, N, K, name, bias=False)
+    p.SA.t.mul_(2.0 ** -12)  # (fp16 holds the results)
+    y = torch.matmul(p.a.double(), p.b.double().t()).float() * (p.sa * 2.0 ** -12)
+    want = (y.double() * p.sb.double().t()).float().to(p.t)
+    assert torch.isfinite(want).all()
+    p.run()
+    assert p.C.holds(want)
+
+
 @pytest.mark.parametrize("M,N,K,name", [(4100, 4099, 130, "bf16"), (4096, 4096, 256, "f32"),
                                         (1000, 50257, 80, "f16"), (8192, 2050, 129, "f32")])
 def test_many_tiles(gpu, M, N, K, name):
