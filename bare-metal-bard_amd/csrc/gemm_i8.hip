@@ -17,7 +17,7 @@
 // (2600 TOP/s; 436-448 on other boxes. The matrix cores are busy 77% of the cycles
 // at about 1.55 of 2.4 GHz: power bounds the clock; on zeros it takes 281).
 // 256 x 256 tiles take a whole CU, so their stores overlap no products: 1000 x 50257 x
-// 768 in fp32 takes 83-88 us, the stores alone 42. 256 x 128 tiles with stages of 64 k,
+// 768 in fp32 takes 83-89 us, the stores alone 42. 256 x 128 tiles with stages of 64 k,
 // two workgroups a CU, took 71 instead of 79 where rows are whole lines, but 59 instead
 // of 54 for 1024 x 49152 in 16 bits and 581 instead of 435 for 8192^3.
 //

@@ -104,8 +104,8 @@ int gemm_get_math(void);
  * with b_scales[n] together with the bias; the result is rounded to `type`. A, B
  * and their strides are multiples of 16 bytes; K is any number: what a row holds
  * behind it has no influence, but up to the next multiple of 16 it is read. C
- * needs its element's alignment (ldc a multiple of 32 and C of 128 bytes are
- * fastest where it is large); what lies between its rows is left as it was. C
+ * needs its element's alignment (rows at multiples of 64 bytes are fastest
+ * where it is large); what lies between its rows is left as it was. C
  * overlaps nothing else. */
 typedef struct GemmI8 {
     int M, N, K;

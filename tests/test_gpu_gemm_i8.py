@@ -112,6 +112,18 @@ def test_many_tiles(gpu, M, N, K, name):
     p.check(p.run())
 
 
+@pytest.mark.parametrize("M,N,K,name,more,skew", [
+    (1000, 50257, 48, "f32", 0, 0), (2304, 7001, 70, "f32", 3, 1), (2304, 6945, 33, "f32", 0, 7),
+    (4096, 8001, 64, "bf16", 0, 0), (4001, 8065, 40, "f16", 5, 3), (256, 57121, 16, "f32", 0, 2),
+    (2100, 7168, 20, "f32", 0, 5), (2304, 7001, 40, "f32", 39, 17)])
+def test_rows_inside_lines(gpu, M, N, K, name, more, skew):
+    """Large results whose rows begin at odd places, or all at the same odd place: every element
+    is stored once, and nothing between the rows."""
+    print("rows inside lines", M, N, K, name, more, skew, flush=True)
+    p = Problem(M, N, K, name, ldc=N + more, skew=skew)
+    p.check(p.run())
+
+
 @pytest.mark.parametrize("stages", list(range(1, 19)) + [25, 40])
 @pytest.mark.parametrize("M,N", [(16, 48), (70, 80), (33, 50257), (2048, 2048), (2100, 2300),
                                  (4096, 4096)])
