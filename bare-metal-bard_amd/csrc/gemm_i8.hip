@@ -56,6 +56,7 @@ struct I8Args {
     int span;   // K of a workgroup (a multiple of 128), or all of it
     int *part;  // span < K: (ranges of K, M, N) sums
     long long part_stride;
+    int first;  // few rows: the launch's first workgroup of the call's
 };
 
 // DA, DB: stages of A and of B in LDS.
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a) {
     const int lane = threadIdx.x & 63, r = lane & 15, quarter = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
-    const int n0 = blockIdx.x * 16;
+    const int n0 = (a.first + (int)blockIdx.x) * 16;
     const int units = (a.K + UNIT - 1) / UNIT, last = (a.K - 1) / CHUNK * CHUNK;
     const int first = (int)((long long)units * wave / waves);
     const int end = (int)((long long)units * (wave + 1) / waves);
@@ -471,8 +472,11 @@ void launch_few(I8Args &a, hipStream_t stream) {
     // Three units of K a wave, up to 16 waves (1 x 50257 x 768: one unit 12.1 us,
     // three 8.5).
     const int waves = std::min(16, std::max(1, ceil_div(ceil_div(a.K, 64), 3)));
-    launch(i8_few_kernel<FM, T>, dim3(ceil_div(a.N, 16)), dim3(64 * waves),
-           waves * FM * 64 * sizeof(i32x4), stream, a);
+    in_launches(ceil_div(a.N, 16), 64 * waves, [&](long long first, unsigned n) {
+        a.first = (int)first;
+        launch(i8_few_kernel<FM, T>, dim3(n), dim3(64 * waves), waves * FM * 64 * sizeof(i32x4),
+               stream, a);
+    });
 }
 
 // C from the sums of the ranges of K: four results a thread.
@@ -662,7 +666,7 @@ int gemm_i8(const GemmI8 *g, hipStream_t stream) {
     }
     const auto go = [&](void *work) {
         I8Args a = {g->A, g->B, g->a_scales, g->b_scales, g->bias, (char *)g->C, g->lda, g->ldb,
-                    g->ldc, g->M, g->N, g->K, 0, 0, 0, (int *)work, 0};
+                    g->ldc, g->M, g->N, g->K, 0, 0, 0, (int *)work, 0, 0};
         if (g->type == BMB_F32)
             launch_i8<float>(a, plan, stream);
         else if (g->type == BMB_F16)
