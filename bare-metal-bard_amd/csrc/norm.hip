@@ -425,24 +425,27 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void grad_kernel(GradArgs a) {
     }
 }
 
-// Wide rows: dinp with a second reading of the row ...
+// Wide rows: dinp with a second reading of the row. A thread adds up to 2^14 terms:
+// in 64 bits (in fp32 their roundings reach 3400 u, u = 2^-24, in rows of 2^24) ...
 template <typename T>
 __global__ __launch_bounds__(1024) void wide_grad_kernel(GradArgs a) {
     constexpr int N = piece_of<T>(), G = 1024;
-    __shared__ float part[G / WAVE];
+    __shared__ double part[G / WAVE];
     const long long row = a.first + blockIdx.x;
     const T *dout = (const T *)a.dout + row * a.dout_stride;
     const T *inp = (const T *)a.inp + row * a.inp_stride;
     const float rstd = a.rstd[row];
-    float dot = 0.0f, w[N], d[N], x[N];
+    float w[N], d[N], x[N];
+    double sum = 0.0;
     for (int c = threadIdx.x * N; c < a.C; c += G * N) {
         load_piece<T, N>(dout, c, a.C, d);
         load_piece<T, N>(inp, c, a.C, x);
         load_piece<float, N>(a.weight, c, a.C, w);
 #pragma unroll
-        for (int e = 0; e < N; ++e) dot = __builtin_fmaf(d[e] * w[e], x[e] * rstd, dot);
+        for (int e = 0; e < N; ++e)
+            sum = __builtin_fma((double)(d[e] * w[e]), (double)(x[e] * rstd), sum);
     }
-    dot = row_all<G>(dot, part, Add()) / a.C;
+    const float dot = (float)(row_all<G>(sum, part, Add()) / a.C);
     for (int c = threadIdx.x * N; c < a.C; c += G * N) {
         float g[N];
         load_piece<T, N>(dout, c, a.C, d);

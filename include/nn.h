@@ -196,9 +196,10 @@ typedef struct RmsNormGrad {
     size_t work_bytes;
 } RmsNormGrad;
 /* dinp = dres + rstd * (dout * weight - xhat * mean(dout * weight * xhat)) with
- * xhat = inp * rstd; dweight += sum_rows dout * xhat. The sums over rows are
- * fp32 over at most 64 rows at a time and 64 bits over those. work: at least
- * rms_norm_backward_workspace() bytes, which need no value; null: the call
+ * xhat = inp * rstd; dweight += sum_rows dout * xhat. The mean is fp32 (37
+ * additions in a chain at most), in 64 bits where C is above 16384. The sums over
+ * rows are fp32 over at most 64 rows at a time and 64 bits over those. work: at
+ * least rms_norm_backward_workspace() bytes, which need no value; null: the call
  * leases from the library's pool, and is refused under graph capture if it
  * needs any. */
 int rms_norm_backward(const RmsNormGrad *grad, struct ihipStream_t *stream);
