@@ -502,23 +502,37 @@ constexpr long long L2_BYTES = 32 << 20;
 // How a product is cut. tile: an index below; ranges: of K.
 struct I8Plan {
     int tile, ranges, span;
-    bool deep;
+    bool deep;  // of tiles of 64 x 64 and 128 x 128: three stages of B
 };
 
-template <typename Tile, typename T>
-void launch_tile(I8Args &a, int ranges, hipStream_t stream) {
+// Tiles at most that are deep (plan_of says why).
+constexpr int DEEP_64 = 768, DEEP_128 = 256;
+
+template <typename Tile>
+dim3 grid_of(I8Args &a, int ranges) {
     a.tiles_m = ceil_div(a.M, Tile::BM);
     a.tiles_n = ceil_div(a.N, Tile::BN);
-    const dim3 grid(a.tiles_m * a.tiles_n * ranges);
-    if (ranges == 1) {
-        // Results that do not fit the L2 caches are stored past them (1000 x 50257 x
-        // 768 in fp32: 94 -> 86 us).
-        const bool past = (long long)a.M * a.N * (int)sizeof(T) > L2_BYTES;
-        launch(past ? i8_kernel<Tile, T, true> : i8_kernel<Tile, T, false>, grid, dim3(Tile::NT), 0,
-               stream, a);
-        return;
+    return dim3(a.tiles_m * a.tiles_n * ranges);
+}
+
+// Results that do not fit the L2 caches are stored past them (1000 x 50257 x 768
+// in fp32: 94 -> 86 us). FIT: they always fit.
+template <typename Tile, typename T, bool FIT>
+void launch_tile(I8Args &a, hipStream_t stream) {
+    const dim3 grid = grid_of<Tile>(a, 1);
+    if constexpr (!FIT) {
+        if ((long long)a.M * a.N * (int)sizeof(T) > L2_BYTES) {
+            launch(i8_kernel<Tile, T, true>, grid, dim3(Tile::NT), 0, stream, a);
+            return;
+        }
     }
-    launch(i8_kernel<Tile, int, false>, grid, dim3(Tile::NT), 0, stream, a);
+    launch(i8_kernel<Tile, T, false>, grid, dim3(Tile::NT), 0, stream, a);
+}
+
+// The sums of each range of K, and what joins them.
+template <typename Tile, typename T>
+void launch_ranges(I8Args &a, int ranges, hipStream_t stream) {
+    launch(i8_kernel<Tile, int, false>, grid_of<Tile>(a, ranges), dim3(Tile::NT), 0, stream, a);
     launch(i8_join_kernel<T>, dim3((unsigned)(((long long)a.M * a.N + 1023) / 1024)), dim3(256), 0,
            stream, a, ranges, FastDiv::of(a.N));
 }
@@ -574,7 +588,8 @@ I8Plan plan_of(int M, int N, int K) {
     // keeps no workgroup from a CU (256 x 4096 x 4096 14.4 -> 10.6 us, 64 x 6400 x 1600
     // 7.9 -> 6.6, 1024 x 4096 x 4096 21.7 -> 19.7; 16 x 50257 x 768, 786 tiles, it would
     // be 9.1 -> 10.6, 2048 x 4096 x 4096 36 -> 38).
-    p.deep = p.tile == TILE_64 ? tiles(64, 64) * p.ranges <= 768 : tiles(128, 128) <= 256;
+    if (p.tile == TILE_64) p.deep = tiles(64, 64) * p.ranges <= DEEP_64;
+    if (p.tile == TILE_128) p.deep = tiles(128, 128) <= DEEP_128;
     return p;
 }
 
@@ -582,16 +597,23 @@ template <typename T>
 void launch_i8(I8Args &a, const I8Plan &p, hipStream_t stream) {
     a.span = p.span;
     a.part_stride = ((long long)a.M * a.N + 3) / 4 * 4;
+    typedef I8Tile<64, 64, 2, 2, 3, 3> Deep64;
+    typedef I8Tile<128, 128, 2, 2, 3, 3> Deep128;
+    static_assert(DEEP_64 * Deep64::BM * Deep64::BN * 4ll <= L2_BYTES &&
+                      DEEP_128 * Deep128::BM * Deep128::BN * 4ll <= L2_BYTES,
+                  "results of deep tiles fit the L2 caches");
     if (p.tile == FEW)
         a.M <= 16 ? launch_few<1, T>(a, stream) : launch_few<2, T>(a, stream);
+    else if (p.ranges > 1)  // (at most 256 workgroups of 64 x 64 tiles)
+        launch_ranges<Deep64, T>(a, p.ranges, stream);
     else if (p.tile == TILE_64)
-        p.deep ? launch_tile<I8Tile<64, 64, 2, 2, 3, 3>, T>(a, p.ranges, stream)
-               : launch_tile<I8Tile<64, 64, 2, 2, 3, 2>, T>(a, p.ranges, stream);
+        p.deep ? launch_tile<Deep64, T, true>(a, stream)
+               : launch_tile<I8Tile<64, 64, 2, 2, 3, 2>, T, false>(a, stream);
     else if (p.tile == TILE_128)
-        p.deep ? launch_tile<I8Tile<128, 128, 2, 2, 3, 3>, T>(a, p.ranges, stream)
-               : launch_tile<I8Tile<128, 128, 2, 2, 3, 2>, T>(a, p.ranges, stream);
+        p.deep ? launch_tile<Deep128, T, true>(a, stream)
+               : launch_tile<I8Tile<128, 128, 2, 2, 3, 2>, T, false>(a, stream);
     else
-        launch_tile<I8Tile<256, 256, 2, 4, 3, 2>, T>(a, p.ranges, stream);
+        launch_tile<I8Tile<256, 256, 2, 4, 3, 2>, T, false>(a, stream);
 }
 
 size_t bytes_of(const I8Plan &p, int M, int N) {
