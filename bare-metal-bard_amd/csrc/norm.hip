@@ -526,22 +526,23 @@ Shape shape_of(int C, int size, int elements) {
     return {0, 0};
 }
 
-// f(G, P) as constants, for P up to MOST.
-template <int MOST, int G, typename F>
+// f(G, P) as constants, for the P from LEAST to MOST that shape_of gives.
+template <int LEAST, int MOST, int G, typename F>
 void with_pieces(int P, F &&f) {
-    if constexpr (MOST > 0) {
+    if constexpr (MOST >= LEAST) {
         if (P == MOST)
             f(std::integral_constant<int, G>(), std::integral_constant<int, MOST>());
         else
-            with_pieces<MOST - 1, G>(P, f);
+            with_pieces<LEAST, MOST - 1, G>(P, f);
     }
 }
+// (G threads have more pieces than MOST times the next smaller G holds)
 template <int MOST, typename F>
 void with_shape(Shape s, F &&f) {
-    if (s.G == 64) with_pieces<MOST, 64>(s.P, f);
-    else if (s.G == 256) with_pieces<MOST, 256>(s.P, f);
-    else if (s.G == 512) with_pieces<MOST, 512>(s.P, f);
-    else with_pieces<MOST, 1024>(s.P, f);
+    if (s.G == 64) with_pieces<1, MOST, 64>(s.P, f);
+    else if (s.G == 256) with_pieces<MOST * 64 / 256 + 1, MOST, 256>(s.P, f);
+    else if (s.G == 512) with_pieces<MOST * 256 / 512 + 1, MOST, 512>(s.P, f);
+    else with_pieces<MOST * 512 / 1024 + 1, MOST, 1024>(s.P, f);
 }
 
 template <typename T, bool NORM, bool I8>

@@ -117,7 +117,9 @@ def kernels(tmp_path_factory):
     return [{name for what, name in got if what == w} for w in ("registered", "launched")]
 
 
-@pytest.mark.parametrize("family", ["i8_kernel", "i8_few_kernel", "i8_join_kernel"])
+@pytest.mark.parametrize("family", ["i8_kernel", "i8_few_kernel", "i8_join_kernel", "rows_kernel",
+                                    "wide_rows_kernel", "grad_kernel", "wide_grad_kernel",
+                                    "wide_sums_kernel", "join_sums_kernel"])
 def test_reached(kernels, family):
     mangled = "_GLOBAL__N_1%d%s" % (len(family), family)
     registered, launched = ({n for n in names if mangled in n} for names in kernels)
