@@ -15,6 +15,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "args.hpp"
 #include "common.hpp"
@@ -130,23 +131,38 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
     }
 }
 
+// Most pairs of a piece: 16 bytes of either half, or of neighbours.
 template <typename T, bool HALF>
-void launch_rotary(RotaryArgs &a, int N, int rest, hipStream_t stream) {
+constexpr int most_pairs() { return 16 / sizeof(T) / (HALF ? 1 : 2); }
+
+// f(N) as a constant, for N from MOST down in halves.
+template <int MOST, typename F>
+void with_pairs(int N, F &&f) {
+    if (N == MOST)
+        f(std::integral_constant<int, MOST>());
+    else if constexpr (MOST > 1)
+        with_pairs<MOST / 2>(N, f);
+}
+
+// rest: elements of a head that are copied.
+template <typename T, bool HALF>
+void launch_rotary(RotaryArgs &a, int rest, hipStream_t stream) {
+    int N = most_pairs<T, HALF>();
+    while (a.pairs % N != 0 || rest % N != 0) N /= 2;
     a.turns = a.heads * (a.pairs / N);
     a.items = a.turns + (rest ? a.heads * (rest / N) : 0);
     a.per_head = FastDiv::of(a.pairs / N);
     a.rest = FastDiv::of(std::max(1, rest / N));
     a.each = std::max(1, THREADS / a.items);
-    const auto kernel = N == 8   ? rotary_kernel<T, HALF, 8>
-                        : N == 4 ? rotary_kernel<T, HALF, 4>
-                        : N == 2 ? rotary_kernel<T, HALF, 2>
-                                 : rotary_kernel<T, HALF, 1>;
-    in_launches(((long long)a.tokens + a.each - 1) / a.each, THREADS,
-                [&](long long first, unsigned n) {
-                    a.first = first;
-                    const size_t lds = a.each * a.pairs * sizeof(float2);
-                    launch(kernel, dim3(n), dim3(THREADS), lds, stream, a);
-                });
+    with_pairs<most_pairs<T, HALF>()>(N, [&](auto pairs) {
+        in_launches(((long long)a.tokens + a.each - 1) / a.each, THREADS,
+                    [&](long long first, unsigned n) {
+                        a.first = first;
+                        const size_t lds = a.each * a.pairs * sizeof(float2);
+                        launch(rotary_kernel<T, HALF, pairs()>, dim3(n), dim3(THREADS), lds, stream,
+                               a);
+                    });
+    });
 }
 
 const char *plan_fault(const Rotary *r) {
@@ -198,17 +214,15 @@ int run(const char *me, const Rotary *r, void *out, long long out_stride, const 
     // What passes is copied, but for in place.
     const int rest = in_place ? 0 : r->head_size - r->dims;
     const bool half = r->layout == BMB_ROTARY_HALF;
-    int N = half && size == 2 ? 8 : half || size == 2 ? 4 : 2;
-    while (a.pairs % N != 0 || rest % N != 0) N /= 2;
     if (type == BMB_F32)
-        half ? launch_rotary<float, true>(a, N, rest, stream)
-             : launch_rotary<float, false>(a, N, rest, stream);
+        half ? launch_rotary<float, true>(a, rest, stream)
+             : launch_rotary<float, false>(a, rest, stream);
     else if (type == BMB_F16)
-        half ? launch_rotary<_Float16, true>(a, N, rest, stream)
-             : launch_rotary<_Float16, false>(a, N, rest, stream);
+        half ? launch_rotary<_Float16, true>(a, rest, stream)
+             : launch_rotary<_Float16, false>(a, rest, stream);
     else
-        half ? launch_rotary<__bf16, true>(a, N, rest, stream)
-             : launch_rotary<__bf16, false>(a, N, rest, stream);
+        half ? launch_rotary<__bf16, true>(a, rest, stream)
+             : launch_rotary<__bf16, false>(a, rest, stream);
     return 0;
 }
 

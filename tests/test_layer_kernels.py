@@ -119,7 +119,7 @@ def kernels(tmp_path_factory):
 
 @pytest.mark.parametrize("family", ["i8_kernel", "i8_few_kernel", "i8_join_kernel", "rows_kernel",
                                     "wide_rows_kernel", "grad_kernel", "wide_grad_kernel",
-                                    "wide_sums_kernel", "join_sums_kernel"])
+                                    "wide_sums_kernel", "join_sums_kernel", "rotary_kernel"])
 def test_reached(kernels, family):
     mangled = "_GLOBAL__N_1%d%s" % (len(family), family)
     registered, launched = ({n for n in names if mangled in n} for names in kernels)
