@@ -246,6 +246,9 @@ int rotary_frequencies(Rotary *r, double base, int scaling, double factor, int t
         return refuse(me, "trained_len is below 1, or not 0 <= slow < fast");
     const double n = r->dims;
     if (scaling == BMB_ROTARY_BASE && r->dims > 2) base *= pow(factor, n / (n - 2.0));
+    // (the last frequency is the farthest from 1)
+    if (!std::isfinite(base) || !std::isfinite(pow(base, 2.0 / n - 1.0)))
+        return refuse(me, "the scaled base or a frequency is not finite");
     for (int i = 0; i < r->dims / 2; ++i) {
         double f = pow(base, -2.0 * i / n);
         if (scaling == BMB_ROTARY_LINEAR) f /= factor;

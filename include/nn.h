@@ -233,7 +233,8 @@ typedef struct Rotary {
                               /* positions: / factor; `fast` times or more: as they are; */
                               /* between: evenly from the one to the other */
 /* Fills plan->freq on the host; launches nothing. factor >= 1; trained_len,
- * slow and fast (0 <= slow < fast) are looked at for BMB_ROTARY_PARTS only. */
+ * slow and fast (0 <= slow < fast) are looked at for BMB_ROTARY_PARTS only. A
+ * scaled base or a frequency that 64 bits do not hold is refused. */
 int rotary_frequencies(Rotary *plan, double base, int scaling, double factor, int trained_len,
                        double slow, double fast);
 /* Turns the first `heads` heads (heads * head_size elements) of each of
