@@ -106,7 +106,7 @@ int gemm_get_math(void);
  * behind it has no influence, but up to the next multiple of 16 it is read. C
  * needs its element's alignment (rows at multiples of 64 bytes are fastest
  * where it is large); what lies between its rows is left as it was. C
- * overlaps nothing else. */
+ * overlaps nothing else. Results in more than 2^22 blocks of 64 x 64 are refused. */
 typedef struct GemmI8 {
     int M, N, K;
     int type; /* of C: BMB_F32 0, BMB_F16 1 or BMB_BF16 2 (nn.h) */

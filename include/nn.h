@@ -153,7 +153,7 @@ int logits_process(void *out, const void *logits, int type, int rows, int V, lon
  * current device, where all buffers live, and return 0, or -1 with a message
  * on stderr, and nothing launched, for arguments they refuse. The structs are
  * host memory, read during the call. Strides are elements from row to row, at
- * least the row's width (0 for an input: one row for all); buffers need their
+ * least the row's width (0 for an input: one row for all), up to 2^40; buffers need their
  * element's alignment only, 16 bytes are fastest. Results overlap neither
  * inputs nor each other unless said so; what lies between rows is left as it
  * was. No result depends on anything but the inputs (no atomics). Nothing is
@@ -237,7 +237,7 @@ typedef struct Rotary {
  * scaled base or a frequency that 64 bits do not hold is refused. */
 int rotary_frequencies(Rotary *plan, double base, int scaling, double factor, int trained_len,
                        double slow, double fast);
-/* Turns the first `heads` heads (heads * head_size elements) of each of
+/* Turns the first `heads` heads (up to 65536; heads * head_size elements) of each of
  * `tokens` rows of `type`: queries and keys of fused QKV rows in one call.
  * positions: (tokens), any number. out may be inp (with its stride). The angle
  * is formed in 64 bits and reduced there. */
