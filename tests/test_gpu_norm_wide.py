@@ -1,5 +1,5 @@
-"""rms_norm_backward of rows of 2^16 to 2^20 elements (include/nn.h): the row's mean is held in 64
-bits, so its bound does not grow with C. u = 2^-24.
+"""rms_norm_backward of wide rows (include/nn.h): many of them a workgroup, and rows of 2^16 to 2^20
+elements, whose mean is held in 64 bits, so that its bound does not grow with C. u = 2^-24.
 
 A term of the mean rounds dout * weight and inp * rstd once each, and the mean rounds to fp32: 3 u
 of the terms' magnitude. What follows rounds at most five times (those two again, the product with
@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from rows_util import TYPES, U, close, half_step, smallest
-from test_gpu_norm import backward, gen, values
+from test_gpu_norm import backward, check_backward, gen, values
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,15 @@ def test_rows(gpu, name):
     dres, weight = torch.randn(3, C, generator=g).to(t), 1.0 + 0.1 * torch.randn(C, generator=g)
     dinp, _, rstd = backward(dout, inp, weight, dres)
     check(dout, inp, weight, dres, dinp, rstd)
+
+
+@pytest.mark.parametrize("name,C", [("f32", 2500), ("bf16", 4100), ("f32", 8200), ("f16", 8200),
+                                    ("bf16", 16400)])
+def test_many_rows(gpu, name, C):
+    """Six rows a workgroup, the last with one: a row's sums are not the next one's."""
+    print("many rows", name, C, flush=True)
+    rows, t, g = 512 * 5 + 9, TYPES[name][1], gen(C)
+    assert rows % 6 == 1
+    inp, dout, dres = (values(rows, C, t, g) for _ in range(3))
+    weight, dw0 = 1.0 + 0.3 * torch.randn(C, generator=g), torch.randn(C, generator=g)
+    check_backward(dout, inp, weight, dres, dw0, backward(dout, inp, weight, dres, dw0))
