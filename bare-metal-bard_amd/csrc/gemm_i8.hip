@@ -14,10 +14,11 @@
 // the stage's start 525 us; spread 510; scales by LDS instead of from memory
 // between the stores, which waited for the stores, 477; A three stages deep 446;
 // results by LDS in whole rows 429; no wait in the loop but for the next stage 423
-// (2600 TOP/s; 436-448 on other boxes. The matrix cores are busy 77% of the cycles
-// at about 1.55 of 2.4 GHz: power bounds the clock; on zeros it takes 281).
+// (2600 TOP/s; up to 448 on other boxes, and 440-515 for the first passes after other
+// work. The matrix cores are busy 77% of the cycles at about 1.55 of 2.4 GHz: power
+// bounds the clock; on zeros it takes 281).
 // 256 x 256 tiles take a whole CU, so their stores overlap no products: 1000 x 50257 x
-// 768 in fp32 takes 83-89 us, the stores alone 42. 256 x 128 tiles with stages of 64 k,
+// 768 in fp32 takes 83-91 us, the stores alone 42. 256 x 128 tiles with stages of 64 k,
 // two workgroups a CU, took 71 instead of 79 where rows are whole lines, but 59 instead
 // of 54 for 1024 x 49152 in 16 bits and 581 instead of 435 for 8192^3.
 //
@@ -469,8 +470,9 @@ __global__ __launch_bounds__(1024) void i8_few_kernel(I8Args a) {
 
 template <int FM, typename T>
 void launch_few(I8Args &a, hipStream_t stream) {
-    // Three units of K a wave, up to 16 waves (1 x 50257 x 768: one unit 12.1 us,
-    // three 8.5).
+    // Three units of K a wave, up to 16 waves. One to eight units are the same within
+    // 4% wherever the rule sends few rows (1 x 2304 x 768 2.63-2.74 us, three 2.69; 1 x 768 x
+    // 6400 5.60-5.74) but for 32 x 2304 x 768: one 3.48, three 3.68, eight 4.12.
     const int waves = std::min(16, std::max(1, ceil_div(ceil_div(a.K, 64), 3)));
     in_launches(ceil_div(a.N, 16), 64 * waves, [&](long long first, unsigned n) {
         a.first = (int)first;
@@ -539,25 +541,48 @@ void launch_ranges(I8Args &a, int ranges, hipStream_t stream) {
 
 enum { FEW, TILE_64, TILE_128, TILE_256 };
 
-// The rule, with times in us of 16-bit results (few rows; 64 x 64, ranges of K in
-// parentheses; 128 x 128; 256 x 256):
-//   1 x 768 x 6400          5.8  (4: 8.5)
-//   32 x 2304 x 768         3.9   4.2 (2: 6.3)
-//   32 x 4096 x 4096        8.4  10.0 (2: 9.4)
-//   32 x 8192 x 768         5.1   4.3 (2: 6.5)
-//   32 x 4096 x 16384      24.9  29.4 (4: 16.1)
-//   1 x 16384 x 16384      49.8  59.6 (8: 57.7)
-//   64 x 4096 x 4096             10.3 (2: 9.8, 4: 9.8)
-//   128 x 1600 x 4800            12.2 (4: 9.4)
-//   256 x 768 x 6400             14.0 (4: 9.9)
-//   512 x 1600 x 6400            14.4 (2: 16.2)
-//   512 x 4096 x 4096            14.9           21    40
-//   1024 x 4096 x 4096           27.5           20    39
-//   2048 x 4096 x 4096           52             36    41
-//   8192 x 2304 x 768            29             25    30
-//   1000 x 50257 x 768           88             76    72
-//   8192 x 6400 x 1600          159            109   102
-//   8192 x 1600 x 6400          128             95    80
+// The rule, and its limits with both sides measured: us of a call among others in a
+// graph, 16-bit results, three sets of operands in turn; * is what the rule takes
+// (64 x 64 and so on: tiles; "in 4": ranges of K, and what joins them).
+//   Few rows, up to 32 where N <= 4096 and K <= 8192, up to 4 where N > 4096 and K >
+//   8192. Rows 1, 4, 16 and 32:
+//                   few rows              64 x 64               64 x 64, split
+//     2304 x 768    2.7* 2.8* 3.0* 3.7*   3.9  4.0  4.0  4.1
+//     4096 x 4096   5.9* 6.1* 6.8* 8.4*   9.9  10.0 10.0 10.1   9.0  9.2  9.4  10.0 in 4
+//     4096 x 8192   8.5* 8.8* 10.3* 14.1*     16.2 16.3 16.4 16.6   11.1 11.4 11.7 12.2 in 4
+//     4096 x 8208   8.1  8.4  9.8  13.5   16.8 17.0 17.1 17.7   11.5* 11.8* 12.2* 12.7* in 4
+//     4096 x 16384  14.0 14.4 17.5 24.1   28.6 29.0 29.2 29.5   15.4* 15.6* 16.0* 16.4* in 4
+//     768 x 16384   12.0 13.0 16.9 24.0   28.0 27.9 27.9 29.0   10.5* 11.1* 11.8* 12.1* in 12
+//     4112 x 768    2.9  3.0  3.4  4.4    4.0* 4.0* 4.1* 4.2*
+//     8192 x 768    3.3  3.4  3.8  4.9    4.1* 4.1* 4.2* 4.2*
+//     8192 x 4096   8.5  8.9  10.2 14.8   10.2* 10.3* 10.4* 10.6*   10.7 10.8 11.0 11.4 in 2
+//     11008 x 4096  11.6 12.2 13.6 20.7   10.5* 10.6* 10.6* 10.9*
+//     16384 x 1600  7.0  6.9  7.9  10.6   7.4* 7.5* 7.7* 7.9*
+//     50257 x 768   8.6  9.3  12.1 17.2   9.1* 9.1* 9.4* 9.8*
+//     8192 x 8192   12.8 13.4 17.2 25.3   16.8 16.9 17.0 17.4   15.0* 15.1* 15.5* 16.2* in 2
+//     8192 x 8208   12.9* 13.3* 15.9 24.2     17.7 17.7 18.0 18.6   15.6 15.7 16.2* 16.8* in 2
+//     16384 x 16384 48.8* 51.9* 73.6 105.6    60.1 60.4 61.0* 61.7*
+//   (N = 4096 and K = 8192 are where 32 rows change sides. One to four rows are faster
+//   as few rows on both sides of either, but for 768 x 16384, 11008 x 4096 and four of
+//   50257 x 768: the limits cost them up to 3.4 us.)
+//   64 x 64 split, from 36 stages on and ten a range:
+//     64 x 2048 x 4480 (35 stages)   10.7*, in 2 10.2, in 4 9.1
+//     64 x 2048 x 4608 (36)          10.7, in 2 10.3, in 3 9.5*, in 4 9.2
+//     64 x 4096 x 4096 (32)          10.4*, in 2 10.4, in 4 10.1
+//     64 x 6400 x 1600 (13)          6.7*, in 2 9.2
+//     128 x 1600 x 4800 (38)         12.3, in 2 11.4, in 3 10.2*, in 4 9.9
+//     256 x 768 x 6400 (50)          14.1, in 2 12.1, in 4 10.2, in 5 10.3*
+//   64 x 64, then 128 x 128 from 192 of these on:
+//     512 x 1600 x 6400 (52 tiles)   14.6*, 22.3
+//     512 x 4096 x 4096 (128)        14.9*, 16.5
+//     768 x 4096 x 4096 (192)        21.5, 17.5*
+//     1024 x 4096 x 4096 (256)       27.3, 19.9*
+//   128 x 128, then 256 x 256 where they fill 70% of their rounds of 256 CUs:
+//     2048 x 4096 x 4096 (50%)       36.6*, 40.7
+//     8192 x 2304 x 768 (56%)        24.6*, 29.1
+//     1000 x 50257 x 768 (77%)       72, 66*
+//     8192 x 1600 x 6400 (88%)       93, 80*
+//     65 x 50257 x 768 (77%)         12.1, 16.8* (rows that a tile wastes are not counted)
 // A tile has to leave few CUs idle; a larger one reads less.
 I8Plan plan_of(int M, int N, int K) {
     I8Plan p = {TILE_64, 1, K, false};
